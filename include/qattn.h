@@ -43,7 +43,8 @@ enum qattn_status {
   QATTN_ERR_ARG = 9         /* other invalid argument */
 };
 
-enum qattn_dtype { QATTN_BF16 = 0, QATTN_FP16 = 1 };
+/* QATTN_F32 and QATTN_I8: the row operators and the INT8 linear only */
+enum qattn_dtype { QATTN_BF16 = 0, QATTN_FP16 = 1, QATTN_F32 = 2, QATTN_I8 = 3 };
 
 /* Q/K scale granularity: the reference's QuantGranularity codes (attn_utils.cuh:41-64) */
 enum qattn_gran {
@@ -514,6 +515,52 @@ int qattn_norm_rope_stats(qattn_seq xq, qattn_seq xk, int dtype, int64_t B, int6
                           const void* wk, const float* cs, const float* sn, int64_t cs_stride, float* rstd_q,
                           float* rstd_k, void* k_mean, void* workspace, size_t workspace_bytes,
                           qattn_stream_t stream);
+
+/*
+ * The row operators around a DiT block, one launch over rows of C channels:
+ *   v = x, or with y: residual_scale * x + gate * p(y), p(y) = y or its norm (post_norm, post_eps, post_weight, post_bias)
+ *   h = v in x's type, contiguous [B, L, C]                                                        (h not null)
+ *   z = norm(v) * weight + bias, then z * (1 + scale) + shift                                      (z not null)
+ * fp32 throughout, v not rounded on its way to z.  x and y: bf16, fp16 or fp32, y of x's type or, beside an fp32 x, of
+ * any; element (b, l, c) at sb * b + sl * l + c.  z: bf16 / fp16 / fp32 contiguous, or QATTN_I8: codes
+ * rint(127 z / max|z|) in rows of z_pitch bytes (a multiple of 16; C .. z_pitch is written 0) and z_scale[b * L + l] =
+ * max|z| / 127.  A row of zeros has scale 0, one with an infinity or a NaN scale NaN and codes 0.  With norm NONE and
+ * neither y nor parameters it is the row quantizer of activations (per token) and of weights (per channel).
+ * Parameters are fp32, bf16 or fp16 with the strides of their broadcast shape (0 along a dimension of one) and
+ * contiguous channels; null: left out.
+ */
+enum qattn_norm { QATTN_NORM_NONE = 0, QATTN_NORM_LAYER = 1, QATTN_NORM_RMS = 2 };
+typedef struct qattn_param {
+  const void* data;
+  int64_t sb, sl;
+  int dtype;
+} qattn_param;
+typedef struct qattn_block_norm_args {
+  size_t size; /* sizeof(qattn_block_norm_args) */
+  const void* x;
+  const void* y;
+  void* h;
+  void* z;
+  float* z_scale;
+  int64_t x_sb, x_sl, y_sb, y_sl, z_pitch;
+  int64_t B, L, C;
+  qattn_param gate, weight, bias, scale, shift, post_weight, post_bias;
+  int x_dtype, y_dtype, z_dtype;
+  int norm, post_norm; /* enum qattn_norm */
+  float eps, post_eps, residual_scale;
+} qattn_block_norm_args;
+int qattn_block_norm(const qattn_block_norm_args* args, qattn_stream_t stream);
+
+/*
+ * INT8 linear: out[m, n] = act(x_scale[m] * w_scale[n] * sum_k x[m, k] w[n, k] + bias[n]), the sum exact in int32.
+ * x [M, K] and w [N, K]: int8 rows of x_pitch / w_pitch bytes, multiples of 16, 16-byte aligned; K a multiple of 128 up
+ * to 131072 (rows are padded with zeros, as qattn_block_norm writes them); codes in [-127, 127].  out: bf16 / fp16 / fp32
+ * rows of out_stride elements.  bias fp32 or null.
+ */
+enum qattn_act { QATTN_ACT_NONE = 0, QATTN_ACT_GELU_TANH = 1, QATTN_ACT_SILU = 2 };
+int qattn_linear_int8(const int8_t* x, int64_t x_pitch, const float* x_scale, const int8_t* w, int64_t w_pitch,
+                      const float* w_scale, const float* bias, void* out, int out_dtype, int64_t out_stride, int64_t M,
+                      int64_t N, int64_t K, int act, qattn_stream_t stream);
 
 #ifdef __cplusplus
 }

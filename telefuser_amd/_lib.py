@@ -17,6 +17,7 @@ LIB_PATH = os.path.join(_HERE, "lib", "libqattn.so")
 
 QATTN_BF16 = 0
 QATTN_FP16 = 1
+QATTN_F32, QATTN_I8 = 2, 3
 QATTN_QUANT_CUDA = 0
 QATTN_QUANT_TRITON = 1
 QATTN_GRAN_BLOCK, QATTN_GRAN_WARP, QATTN_GRAN_THREAD = 1, 2, 3
@@ -52,6 +53,8 @@ EXPORTED = (
     "qattn_quant_qk_varlen_int8",
     "qattn_v_tile_half_varlen",
     "qattn_fwd_varlen",
+    "qattn_block_norm",
+    "qattn_linear_int8",
 )
 
 
@@ -59,6 +62,23 @@ class QattnSeq(ctypes.Structure):
     """struct qattn_seq: element (b, l, h, d) at data[b*sb + l*sl + h*sh + d]."""
 
     _fields_ = [("data", ctypes.c_void_p), ("sb", ctypes.c_int64), ("sl", ctypes.c_int64), ("sh", ctypes.c_int64)]
+
+
+class QattnParam(ctypes.Structure):
+    """struct qattn_param: a parameter with the strides of its broadcast shape."""
+
+    _fields_ = [("data", ctypes.c_void_p), ("sb", ctypes.c_int64), ("sl", ctypes.c_int64), ("dtype", ctypes.c_int)]
+
+
+class QattnBlockNormArgs(ctypes.Structure):
+    """struct qattn_block_norm_args."""
+
+    _fields_ = (
+        [("size", ctypes.c_size_t)] + [(n, ctypes.c_void_p) for n in ("x", "y", "h", "z", "z_scale")] +
+        [(n, ctypes.c_int64) for n in ("x_sb", "x_sl", "y_sb", "y_sl", "z_pitch", "B", "L", "C")] +
+        [(n, QattnParam) for n in ("gate", "weight", "bias", "scale", "shift", "post_weight", "post_bias")] +
+        [(n, ctypes.c_int) for n in ("x_dtype", "y_dtype", "z_dtype", "norm", "post_norm")] +
+        [(n, ctypes.c_float) for n in ("eps", "post_eps", "residual_scale")])
 
 
 class QattnError(RuntimeError):
@@ -165,6 +185,10 @@ def load() -> ctypes.CDLL:
     L.qattn_v_tile_half_varlen.argtypes = [S, i32, i64, i64, i64, i64, i64, vp, vp, vp, i64, vp]
     L.qattn_fwd_varlen.argtypes = [S, vp, S, vp, vp, i64, S, i32, i64, i64, i64, i64, i64, i64, i64, i64, f32, i32, vp,
                                    vp, vp, vp, vp, vp]
+    L.qattn_block_norm.argtypes = [ctypes.POINTER(QattnBlockNormArgs), vp]
+    L.qattn_linear_int8.argtypes = [vp, i64, vp, vp, i64, vp, vp, vp, i32, i64, i64, i64, i64, i32, vp]
+    for name in ("qattn_block_norm", "qattn_linear_int8"):
+        getattr(L, name).restype = i32
     for name in ("qattn_norm_rope_stats", "qattn_sage_quant_half", "qattn_lse_finish", "qattn_v_tile_half_ex", "qattn_v_tile_half_varlen_ex", "qattn_varlen_offsets", "qattn_quant_qk_varlen_int8", "qattn_v_tile_half_varlen",
                  "qattn_fwd_varlen"):
         getattr(L, name).restype = i32
@@ -210,3 +234,21 @@ def dtype_code(dt: torch.dtype) -> int:
 
 def stream_of(t: torch.Tensor):
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+class _Here:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE_DEVICE = _Here()
+
+
+def on_device(dev: torch.device):
+    """Context in which a launch on a stream of dev is valid: dev made current, unless it is already."""
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        return _HERE_DEVICE
+    return torch.cuda.device(dev)

@@ -130,10 +130,36 @@ __device__ __forceinline__ void varlen_range(const int32_t* cu, int64_t b, int64
   len = min(s1 - s0, maxlen);
 }
 
+// Row quantization of the INT8 projections from the bits of max|x| (sign cleared): scale = max|x| / 127 and code =
+// rint(127 x / max|x|), the quotient correctly rounded, so that the codes of half values are those of the real
+// numbers.  A row of zeros has scale 0 and codes 0.  A row with an infinity or a NaN has scale NaN and codes 0: every
+// product with it is NaN.  Rows of maximum below 1e-30 are scaled up first, where the quotient's corrections would
+// underflow.
+struct RowQuant {
+  float scale, pre, mult, top, rcp;
+  __device__ __forceinline__ explicit RowQuant(uint32_t top_bits) {
+    const float t = __uint_as_float(top_bits);
+    const bool fine = top_bits != 0 && top_bits < 0x7f800000u;
+    scale = top_bits < 0x7f800000u ? t / 127.0f : __uint_as_float(0x7fc00000u);
+    pre = t < 1e-30f ? 0x1p80f : t > 1e30f ? 0x1p-40f : 1.0f;
+    mult = fine ? 127.0f : 0.0f;
+    top = fine ? t * pre : 1.0f;
+    rcp = refined_rcp(top);
+  }
+  __device__ __forceinline__ int code(float x) const {
+    return cvt_i32_trunc_sat(__builtin_rintf(div_by(x * pre * mult, top, rcp)));
+  }
+};
+
 // wave64 reductions (DPP / permute through the compiler's shuffle lowering)
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
   return v;
 }
 __device__ __forceinline__ float wave_sum(float v) {
