@@ -136,18 +136,29 @@ __device__ __forceinline__ void varlen_range(const int32_t* cu, int64_t b, int64
 // product with it is NaN.  Rows of maximum below 1e-30 are scaled up first, where the quotient's corrections would
 // underflow.
 struct RowQuant {
-  float scale, pre, mult, top, rcp;
+  float scale, mult, top, rcp;
+  bool fine;
   __device__ __forceinline__ explicit RowQuant(uint32_t top_bits) {
     const float t = __uint_as_float(top_bits);
-    const bool fine = top_bits != 0 && top_bits < 0x7f800000u;
+    fine = top_bits != 0 && top_bits < 0x7f800000u;
     scale = top_bits < 0x7f800000u ? t / 127.0f : __uint_as_float(0x7fc00000u);
-    pre = t < 1e-30f ? 0x1p80f : t > 1e30f ? 0x1p-40f : 1.0f;
-    mult = fine ? 127.0f : 0.0f;
+    const float pre = t < 1e-30f ? 0x1p80f : t > 1e30f ? 0x1p-40f : 1.0f;
+    mult = 127.0f * pre;
     top = fine ? t * pre : 1.0f;
     rcp = refined_rcp(top);
   }
-  __device__ __forceinline__ int code(float x) const {
-    return cvt_i32_trunc_sat(__builtin_rintf(div_by(x * pre * mult, top, rcp)));
+  // the code in the low byte.  127 x is exact for half values; its quotient takes one correction (as quant_code_triton's),
+  // and adding 1.5 * 2^23 rounds it to an integer, ties to even, in the low bits
+  __device__ __forceinline__ uint32_t code(float x) const {
+    const float n = x * mult;
+    const float q = n * rcp;
+    return __float_as_uint(fmaf(fmaf(-top, q, n), rcp, q) + 12582912.0f);
+  }
+  // four codes, the first in the low byte
+  __device__ __forceinline__ uint32_t code4(float a, float b, float c, float d) const {
+    const uint32_t lo = __builtin_amdgcn_perm(code(b), code(a), 0x0c0c0400u);
+    const uint32_t hi = __builtin_amdgcn_perm(code(d), code(c), 0x0c0c0400u);
+    return fine ? lo | hi << 16 : 0u;
   }
 };
 
@@ -157,15 +168,35 @@ __device__ __forceinline__ float wave_max(float v) {
   for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
   return v;
 }
-__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
-  return v;
-}
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
+}
+
+// The same over the DPP network, the result in a scalar register: within quads, rows of 16 (half mirror, mirror), then
+// lane 15 of each row to the next one and lane 31 to the upper half; lane 63 ends with the whole wave's.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp(uint32_t old, uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)old, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <typename OP>
+__device__ __forceinline__ uint32_t wave_reduce(uint32_t v, uint32_t zero, OP op) {
+  v = op(v, dpp<0xb1, 0xf>(zero, v));
+  v = op(v, dpp<0x4e, 0xf>(zero, v));
+  v = op(v, dpp<0x141, 0xf>(zero, v));
+  v = op(v, dpp<0x140, 0xf>(zero, v));
+  v = op(v, dpp<0x142, 0xa>(zero, v));
+  v = op(v, dpp<0x143, 0xc>(zero, v));
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ float wave_total(float v) {
+  return __uint_as_float(wave_reduce(__float_as_uint(v), 0u, [](uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }));
+}
+__device__ __forceinline__ uint32_t wave_top(uint32_t v) {
+  return wave_reduce(v, 0u, [](uint32_t a, uint32_t b) { return max(a, b); });
 }
 
 }  // namespace qattn

@@ -109,18 +109,25 @@ def test_strides_alignment_and_types(C):
     views = {"rows apart": big[:, 1:L + 1, :C], "off 16 bytes": big[:, :L, 1:C + 1], "odd rows": big[:, 0:2 * 3:2, 8:C + 8],
              "channels apart": big[:, :L, 0:2 * C:2], "batch first": big.transpose(0, 1)[:, :, :C],
              "one batch entry": big[1, :L, 8:C + 8], "repeated row": big[:, :1, :C].expand(B, L, C)}
+    # the same float64 tolerance as everywhere, not the bits of the contiguous call: how a row lies in memory decides which
+    # lane sums which of its channels, and float32 sums in another order differ within the counted roundings
+    def same(z, what, x, y=None, h=None, **how):
+        rh, eh, rz, ez = P.block(x, y, **how)
+        P.check(z, rz, ez, f"z {what}")
+        if h is not None:
+            P.check(h, rh, eh, f"h {what}")
+
     for what, v in views.items():
-        assert torch.equal(block_norm(v), block_norm(v.contiguous())), what
+        same(block_norm(v), what, v)
         h, z = gated_residual_norm(v, v, norm="rms")
-        hc, zc = gated_residual_norm(v.contiguous(), v.contiguous(), norm="rms")
-        assert torch.equal(h, hc) and torch.equal(z, zc), what
+        same(z, what, v, v, h, norm_kind="rms")
     flat = torch.zeros(B * L * C + 8, dtype=FP32, device="cuda")
     off = flat[1:1 + B * L * C].view(B, L, C)
     off.copy_(_x((B, L, C), 4, FP32))
-    assert torch.equal(block_norm(off), block_norm(off.clone()))
+    same(block_norm(off), "off 4 bytes", off)
     x = _x((B, L, C), 5, FP32)
     odd = _p((C + 1,), 6)[1:]  # a parameter off 16 bytes
-    assert torch.equal(block_norm(x, odd), block_norm(x, odd.clone()))
+    same(block_norm(x, odd), "odd parameter", x, weight=odd)
     for yt, zt in itertools.product((BF16, FP16, FP32), (BF16, FP16, FP32)):  # a float32 residual stream
         y = _x((B, L, C), 6, yt)
         h, z = gated_residual_norm(x, y, out_dtype=zt)
