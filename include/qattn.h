@@ -555,12 +555,24 @@ int qattn_block_norm(const qattn_block_norm_args* args, qattn_stream_t stream);
  * INT8 linear: out[m, n] = act(x_scale[m] * w_scale[n] * sum_k x[m, k] w[n, k] + bias[n]), the sum exact in int32.
  * x [M, K] and w [N, K]: int8 rows of x_pitch / w_pitch bytes, multiples of 16, 16-byte aligned; K a multiple of 128 up
  * to 131072 (rows are padded with zeros, as qattn_block_norm writes them); codes in [-127, 127].  out: bf16 / fp16 / fp32
- * rows of out_stride elements.  bias fp32 or null.
+ * rows of out_stride elements.  bias fp32 or null.  Workspace (16-byte aligned, no contents kept; 0 bytes for most sizes):
+ * the int32 sums of a product split along K.
  */
+size_t qattn_linear_int8_workspace_size(int64_t M, int64_t N, int64_t K);
 enum qattn_act { QATTN_ACT_NONE = 0, QATTN_ACT_GELU_TANH = 1, QATTN_ACT_SILU = 2 };
 int qattn_linear_int8(const int8_t* x, int64_t x_pitch, const float* x_scale, const int8_t* w, int64_t w_pitch,
                       const float* w_scale, const float* bias, void* out, int out_dtype, int64_t out_stride, int64_t M,
-                      int64_t N, int64_t K, int act, qattn_stream_t stream);
+                      int64_t N, int64_t K, int act, void* workspace, size_t workspace_bytes, qattn_stream_t stream);
+/*
+ * The same from floating rows: x [B, L, cols] (bf16 / fp16 / fp32, element strides, contiguous channels), quantized as
+ * qattn_block_norm does and with the same bits; w rows of at least cols rounded up to 128 bytes.  The INT8 rows go to the
+ * workspace (16-byte aligned, no contents kept; a few tokens need none).
+ */
+size_t qattn_linear_int8_rows_workspace_size(int64_t M, int64_t N, int64_t cols);
+int qattn_linear_int8_rows(const void* x, int x_dtype, int64_t x_sb, int64_t x_sl, int64_t B, int64_t L, int64_t cols,
+                           const int8_t* w, int64_t w_pitch, const float* w_scale, const float* bias, void* out,
+                           int out_dtype, int64_t out_stride, int64_t N, int act, void* workspace, size_t workspace_bytes,
+                           qattn_stream_t stream);
 
 #ifdef __cplusplus
 }

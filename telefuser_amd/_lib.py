@@ -7,6 +7,7 @@ raises, so the HIP kernels are always what runs.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -54,7 +55,10 @@ EXPORTED = (
     "qattn_v_tile_half_varlen",
     "qattn_fwd_varlen",
     "qattn_block_norm",
+    "qattn_linear_int8_workspace_size",
     "qattn_linear_int8",
+    "qattn_linear_int8_rows_workspace_size",
+    "qattn_linear_int8_rows",
 )
 
 
@@ -186,8 +190,14 @@ def load() -> ctypes.CDLL:
     L.qattn_fwd_varlen.argtypes = [S, vp, S, vp, vp, i64, S, i32, i64, i64, i64, i64, i64, i64, i64, i64, f32, i32, vp,
                                    vp, vp, vp, vp, vp]
     L.qattn_block_norm.argtypes = [ctypes.POINTER(QattnBlockNormArgs), vp]
-    L.qattn_linear_int8.argtypes = [vp, i64, vp, vp, i64, vp, vp, vp, i32, i64, i64, i64, i64, i32, vp]
-    for name in ("qattn_block_norm", "qattn_linear_int8"):
+    L.qattn_linear_int8_workspace_size.argtypes = [i64, i64, i64]
+    L.qattn_linear_int8_workspace_size.restype = sz
+    L.qattn_linear_int8.argtypes = [vp, i64, vp, vp, i64, vp, vp, vp, i32, i64, i64, i64, i64, i32, vp, sz, vp]
+    L.qattn_linear_int8_rows_workspace_size.argtypes = [i64, i64, i64]
+    L.qattn_linear_int8_rows_workspace_size.restype = sz
+    L.qattn_linear_int8_rows.argtypes = [vp, i32, i64, i64, i64, i64, i64, vp, i64, vp, vp, vp, i32, i64, i64, i32, vp,
+                                         sz, vp]
+    for name in ("qattn_block_norm", "qattn_linear_int8", "qattn_linear_int8_rows"):
         getattr(L, name).restype = i32
     for name in ("qattn_norm_rope_stats", "qattn_sage_quant_half", "qattn_lse_finish", "qattn_v_tile_half_ex", "qattn_v_tile_half_varlen_ex", "qattn_varlen_offsets", "qattn_quant_qk_varlen_int8", "qattn_v_tile_half_varlen",
                  "qattn_fwd_varlen"):
@@ -236,19 +246,17 @@ def stream_of(t: torch.Tensor):
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
 
 
-class _Here:
-    def __enter__(self):
-        return self
 
-    def __exit__(self, *exc):
-        return False
+def raw_stream(index: int) -> int:
+    """The handle of the current stream of GPU ``index`` (stream_of without building a Stream object)."""
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
-_HERE_DEVICE = _Here()
+_HERE_DEVICE = contextlib.nullcontext()
 
 
-def on_device(dev: torch.device):
-    """Context in which a launch on a stream of dev is valid: dev made current, unless it is already."""
-    if dev.index is None or dev.index == torch.cuda.current_device():
+def on_device(index: int):
+    """Context in which a launch on a stream of GPU ``index`` is valid: it is made current, unless it is already."""
+    if index == torch._C._cuda_getDevice():
         return _HERE_DEVICE
-    return torch.cuda.device(dev)
+    return torch.cuda.device(index)

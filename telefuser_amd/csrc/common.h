@@ -199,4 +199,13 @@ __device__ __forceinline__ uint32_t wave_top(uint32_t v) {
   return wave_reduce(v, 0u, [](uint32_t a, uint32_t b) { return max(a, b); });
 }
 
+// of each half wave, in its last lane
+__device__ __forceinline__ uint32_t half_wave_top(uint32_t v) {
+  v = max(v, dpp<0xb1, 0xf>(0u, v));
+  v = max(v, dpp<0x4e, 0xf>(0u, v));
+  v = max(v, dpp<0x141, 0xf>(0u, v));
+  v = max(v, dpp<0x140, 0xf>(0u, v));
+  return max(v, dpp<0x142, 0xa>(0u, v));
+}
+
 }  // namespace qattn

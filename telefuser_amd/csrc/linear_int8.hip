@@ -42,6 +42,8 @@ struct LinearParams {
   int64_t M, N;
   int K, act;
   int tiles_m, tiles_n;
+  v4i* part;         // split along K: [splits, tiles, 8 waves, NI * MJ, 64 lanes]
+  int split_stages;  // stages of a split
 };
 
 constexpr int kLinK = 128;  // bytes of K per stage
@@ -97,6 +99,19 @@ __device__ __forceinline__ void store_out8(char* o, int dtype, bool vec, int64_t
     }
 }
 
+template <int TM, int TN>
+__device__ __forceinline__ void place_tile(const LinearParams& p, int slot, int tiles, int64_t& m0, int64_t& n0) {
+  const uint32_t id = (uint32_t)xcd_remap(slot, tiles);
+  const uint32_t per = kLinGroup * p.tiles_n, g = id / per, in = id - g * per;
+  const uint32_t gm = min((uint32_t)kLinGroup, (uint32_t)p.tiles_m - g * kLinGroup);
+  const uint32_t tn = in / gm;
+  m0 = (int64_t)(g * kLinGroup + in - tn * gm) * TM;
+  n0 = (int64_t)tn * TN;
+}
+
+// ACT = kSplit: a workgroup multiplies split_stages stages of a tile and leaves the int32 sums in p.part, each register of
+// the wave as one 1 KiB line.
+constexpr int kSplit = -1;
 template <int TM, int TN, int NB, int ACT>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void linear_int8_kernel(LinearParams p) {
   constexpr int WM = 2, WN = 4, kWaves = WM * WN;
@@ -122,18 +137,16 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   for (int i = 0; i < IW; i++) vw[i] = (uint32_t)(channel((i * kWaves + wave) * 8 + (lane >> 3)) * p.w_pitch) + chunk;
 
   const int tiles = p.tiles_m * p.tiles_n;
-  auto place = [&](int slot, int64_t& m0, int64_t& n0) {
-    const uint32_t id = (uint32_t)xcd_remap(slot, tiles);
-    const uint32_t per = kLinGroup * p.tiles_n, g = id / per, in = id - g * per;
-    const uint32_t gm = min((uint32_t)kLinGroup, (uint32_t)p.tiles_m - g * kLinGroup);
-    const uint32_t tn = in / gm;
-    m0 = (int64_t)(g * kLinGroup + in - tn * gm) * TM;
-    n0 = (int64_t)tn * TN;
-  };
+  auto place = [&](int slot, int64_t& m0, int64_t& n0) { place_tile<TM, TN>(p, slot, tiles, m0, n0); };
 
+  constexpr bool kWhole = ACT != kSplit;
+  const int split = kWhole ? 0 : blockIdx.x / tiles;
+  const int slot0 = kWhole ? blockIdx.x : blockIdx.x - split * tiles, stride = kWhole ? gridDim.x : tiles;
+  const uint32_t k0 = kWhole ? 0 : (uint32_t)(split * p.split_stages * kLinK);
+  const uint32_t k1 = kWhole ? (uint32_t)p.K : min((uint32_t)p.K, k0 + p.split_stages * kLinK);
   // where the DMA stands: the tile in slot fslot (the fn-th of this workgroup), byte fk of its rows
-  int fslot = blockIdx.x, fn = 0;
-  uint32_t fk = 0;
+  int fslot = slot0, fn = 0;
+  uint32_t fk = k0;
   v4u rx, rw;
   auto enter = [&]() {
     if (fslot >= tiles) {
@@ -145,6 +158,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     const int64_t rm = min((int64_t)TM, p.M - m0), rn = min((int64_t)TN, p.N - n0);
     rx = make_rsrc(p.x + m0 * p.x_pitch, (uint32_t)((rm - 1) * p.x_pitch + p.K));
     rw = make_rsrc(p.w + n0 * p.w_pitch, (uint32_t)((rn - 1) * p.w_pitch + p.K));
+    if constexpr (!kWhole) return;
     const v4u rs = make_rsrc(p.w_scale + n0, (uint32_t)rn * 4), rt = make_rsrc(p.x_scale + m0, (uint32_t)rm * 4);
     const v4u rb = make_rsrc(p.bias ? p.bias + n0 : p.w_scale, p.bias ? (uint32_t)rn * 4 : 0u);
     const uint32_t to = base + NB * kStage + (fn & 3) * kVec;
@@ -156,8 +170,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   };
   auto advance = [&]() {
     fk += kLinK;
-    if (fk == (uint32_t)p.K) {
-      fk = 0, fslot += gridDim.x, fn++;
+    if (fk == k1) {
+      fk = k0, fslot += stride, fn++;
       enter();
     }
   };
@@ -186,10 +200,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
   for (int r = 0; r < NR; r++) read(0, 0, r, a[0], b[0]);
 
-  const int steps = p.K / kLinK;
+  const int steps = (k1 - k0) / kLinK;
   uint32_t cur = 0;
   int n = 0;
-  for (int slot = blockIdx.x; slot < tiles; slot += gridDim.x, n++) {
+  for (int slot = slot0; slot < tiles; slot += stride, n++) {
     v4i acc[NI][MJ];
 #pragma unroll
     for (int i = 0; i < NI; i++)
@@ -234,6 +248,15 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 
     int64_t m0, n0;
     place(slot, m0, n0);
+    if constexpr (!kWhole) {
+      v4i* to = p.part + (((int64_t)split * tiles + slot) * kWaves + wave) * (NM * 64) + lane;
+#pragma unroll
+      for (int j = 0; j < MJ; j++)
+        if (m0 + wm * (TM / WM) + j * 16 < p.M)
+#pragma unroll
+          for (int i = 0; i < NI; i++) to[(j * NI + i) * 64] = acc[i][j];
+      continue;
+    }
     const float* vec = reinterpret_cast<const float*>(lds + NB * kStage + (n & 3) * kVec);
     const int cl = wn * (TN / WN) + (lane >> 4) * 8, ml = wm * (TM / WM) + row;
     const int es = p.out_dtype == QATTN_F32 ? 4 : 2;
@@ -258,9 +281,211 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
+// The sums of the splits of a 128 x 128 tile, and what the tile kernel does with them at its end.  A wave takes what one
+// wave of the tile kernel left of 16 tokens.
+template <int ACT>
+__global__ __launch_bounds__(256) void linear_join_kernel(LinearParams p, int splits) {
+  constexpr int TM = 128, TN = 128, WM = 2, WN = 4, NI = TN / WN / 16, MJ = TM / WM / 16;
+  const int lane = threadIdx.x & 63, id = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int tiles = p.tiles_m * p.tiles_n;
+  const int j = id % MJ, wave = id / MJ % 8, slot = id / (MJ * 8);
+  if (slot >= tiles) return;
+  int64_t m0, n0;
+  place_tile<TM, TN>(p, slot, tiles, m0, n0);
+  m0 += wave % WM * (TM / WM) + j * 16;
+  n0 += wave / WM * (TN / WN) + (lane >> 4) * 8;
+  if (m0 >= p.M) return;
+  const v4i* from = p.part + ((int64_t)slot * 8 + wave) * (NI * MJ * 64) + j * NI * 64 + lane;
+  v4i sum[NI]{};
+#pragma unroll 4
+  for (int s = 0; s < splits; s++)
+#pragma unroll
+    for (int i = 0; i < NI; i++) sum[i] += from[(int64_t)s * tiles * 8 * NI * MJ * 64 + i * 64];
+  const int64_t m = m0 + (lane & 15), left = p.N - n0;
+  if (m >= p.M) return;
+  const float sx = p.x_scale[m];
+  const int es = p.out_dtype == QATTN_F32 ? 4 : 2;
+  float y[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++)
+    y[e] = e < left ? activate<ACT>(fmaf((float)sum[e / 4][e % 4] * sx, p.w_scale[n0 + e], p.bias ? p.bias[n0 + e] : 0.0f))
+                    : 0.0f;
+  store_out8(static_cast<char*>(p.out) + (m * p.out_stride + n0) * es, p.out_dtype, p.out_vec, left, y);
+}
+
+// ------------------------------------------------------------------------------------------------
+// few tokens
+// ------------------------------------------------------------------------------------------------
+// Up to 16 tokens the weight is what there is to read.  A workgroup takes 16 NI channels and all tokens; its eight waves
+// take turns along K, 128 bytes a turn, and read the weight's fragments straight from global memory, whole lines, several
+// turns ahead.  Their sums meet in LDS.  X: a floating x is quantized by every workgroup for itself, with the code of the
+// row quantizer and so to the same bits, which saves the quantizer's launch and the rows' way through memory; for up to
+// kFewValues values, where that costs less than the launch.
+constexpr int kFewRows = 16;
+constexpr int kFewValues = 16384;
+
+struct FewParams {
+  LinearParams lin;  // x and x_scale: the INT8 rows (X < 0)
+  const void* x;     // the floating rows, L of them to a batch entry
+  int64_t xb, xl;
+  int L, cols;
+  bool vec;  // four values in a load
+};
+
+template <int X>
+__device__ __forceinline__ void few_values4(const void* x, int64_t at, int left, bool vec, float (&v)[4]) {
+  if constexpr (X == QATTN_F32) {
+    const float* q = static_cast<const float*>(x) + at;
+    if (vec && left >= 4) {
+      const v4f r = *reinterpret_cast<const v4f*>(q);
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[e] = r[e];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[e] = e < left ? q[e] : 0.0f;
+    }
+  } else {
+    const uint16_t* q = static_cast<const uint16_t*>(x) + at;
+    uint16_t h[4];
+    if (vec && left >= 4) {
+      const v2u r = *reinterpret_cast<const v2u*>(q);
+      __builtin_memcpy(h, &r, 8);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++) h[e] = e < left ? q[e] : (uint16_t)0;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = half_to_f32<X == QATTN_FP16>(h[e]);
+  }
+}
+
+// X: element type of the floating x, or -1 for INT8 rows.
+template <int NI, int X, int ACT>
+__global__ __launch_bounds__(512) void linear_few_kernel(FewParams f) {
+  const LinearParams& p = f.lin;
+  constexpr int kWaves = 8, kAhead = 4 / NI;
+  __shared__ __attribute__((aligned(16))) v4i part[kWaves][NI][64];
+  __shared__ __attribute__((aligned(16))) uint8_t rows[X < 0 ? 16 : kFewValues + 16 * 16];  // 16 bytes apart: banks
+  __shared__ uint32_t tops[16];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t n0 = (int64_t)blockIdx.x * 16 * NI;
+  const int M = (int)p.M, K = p.K;
+
+  // the weight's first lines are under way while the rows are quantized
+  const int8_t* w[NI];
+#pragma unroll
+  for (int i = 0; i < NI; i++) w[i] = p.w + min(n0 + i * 16 + (lane & 15), p.N - 1) * p.w_pitch + (lane >> 4) * 16;
+  v4i a[kAhead][NI][2];
+  auto load = [&](int k, v4i (&a)[NI][2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NI; i++) {
+      a[i][0] = *reinterpret_cast<const v4i*>(w[i] + k);
+      a[i][1] = *reinterpret_cast<const v4i*>(w[i] + k + 64);
+    }
+  };
+  constexpr int kTurn = kWaves * kLinK;
+#pragma unroll
+  for (int i = 0; i < kAhead; i++)
+    if (wave * kLinK + i * kTurn < K) load(wave * kLinK + i * kTurn, a[i]);
+  // and the scales of the four channels a lane ends with
+  const int64_t c = n0 + wave * 16 + (lane >> 4) * 4;
+  float sw[4], bias[4];
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const bool in = wave < NI && c + e < p.N;
+    sw[e] = in ? p.w_scale[c + e] : 0.0f;
+    bias[e] = in && p.bias ? p.bias[c + e] : 0.0f;
+  }
+
+  const int pitch = K + 16;
+  if constexpr (X >= 0) {
+    // words of four values; 32 of them lie in one row
+    constexpr int kWords = kFewValues / 4 / 512;
+    const int per = K / 4, words = M * per;
+    float v[kWords][4];
+    int at[kWords], of[kWords];
+    if (threadIdx.x < 16) tops[threadIdx.x] = 0;
+#pragma unroll
+    for (int i = 0; i < kWords; i++) {
+      const int id = threadIdx.x + i * 512;
+      of[i] = id < words ? id / per : -1;
+      if (of[i] < 0) continue;
+      const int c = (id - of[i] * per) * 4, b = of[i] / f.L;
+      at[i] = of[i] * pitch + c;
+      few_values4<X>(f.x, b * f.xb + (of[i] - b * f.L) * f.xl + c, f.cols - c, f.vec, v[i]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWords; i++) {
+      uint32_t top = 0;
+      if (of[i] >= 0)
+#pragma unroll
+        for (int e = 0; e < 4; e++) top = max(top, __float_as_uint(v[i][e]) & 0x7fffffffu);
+      top = half_wave_top(top);
+      if ((lane & 31) == 31 && of[i] >= 0) atomicMax(&tops[of[i]], top);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWords; i++)
+      if (of[i] >= 0)
+        *reinterpret_cast<uint32_t*>(rows + at[i]) = RowQuant(tops[of[i]]).code4(v[i][0], v[i][1], v[i][2], v[i][3]);
+    __syncthreads();
+  }
+  const int64_t m = min(lane & 15, M - 1);  // tokens past the last repeat it and are dropped
+  const int8_t* x = X >= 0 ? reinterpret_cast<const int8_t*>(rows) + m * pitch + (lane >> 4) * 16
+                           : p.x + m * p.x_pitch + (lane >> 4) * 16;
+  v4i acc[NI]{};
+  for (int k0 = wave * kLinK; k0 < K; k0 += kAhead * kTurn) {
+#pragma unroll
+    for (int i = 0; i < kAhead; i++) {
+      const int k = k0 + i * kTurn;
+      if (k < K) {
+        const v4i b0 = *reinterpret_cast<const v4i*>(x + k), b1 = *reinterpret_cast<const v4i*>(x + k + 64);
+#pragma unroll
+        for (int n = 0; n < NI; n++) {
+          acc[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i][n][0], b0, acc[n], 0, 0, 0);
+          acc[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[i][n][1], b1, acc[n], 0, 0, 0);
+        }
+        if (k + kAhead * kTurn < K) load(k + kAhead * kTurn, a[i]);
+      }
+    }
+  }
+#pragma unroll
+  for (int n = 0; n < NI; n++) part[wave][n][lane] = acc[n];
+  __syncthreads();
+  // a wave finishes 16 channels: four a lane
+  if (wave >= NI || (lane & 15) >= M) return;
+  v4i sum = part[0][wave][lane];
+#pragma unroll
+  for (int i = 1; i < kWaves; i++) sum += part[i][wave][lane];
+  const float sx = X >= 0 ? RowQuant(tops[m]).scale : p.x_scale[m];
+#pragma unroll
+  for (int e = 0; e < 4; e++)
+    if (c + e < p.N) {
+      const float y = activate<ACT>(fmaf((float)sum[e] * sx, sw[e], bias[e]));
+      const int64_t at = m * p.out_stride + c + e;
+      if (p.out_dtype == QATTN_F32) static_cast<float*>(p.out)[at] = y;
+      else static_cast<uint16_t*>(p.out)[at] = p.out_dtype == QATTN_FP16 ? f32_to_f16(y) : f32_to_bf16(y);
+    }
+}
+
 }  // namespace qattn
 
 using namespace qattn;
+
+template <int NI, int X>
+static int launch_few(const FewParams& f, hipStream_t stream) {
+  const dim3 grid((unsigned)((f.lin.N + 16 * NI - 1) / (16 * NI))), block(512);
+  if (f.lin.act == QATTN_ACT_GELU_TANH) linear_few_kernel<NI, X, QATTN_ACT_GELU_TANH><<<grid, block, 0, stream>>>(f);
+  else if (f.lin.act == QATTN_ACT_SILU) linear_few_kernel<NI, X, QATTN_ACT_SILU><<<grid, block, 0, stream>>>(f);
+  else linear_few_kernel<NI, X, QATTN_ACT_NONE><<<grid, block, 0, stream>>>(f);
+  return check_launch("linear_int8");
+}
+template <int X>
+static int launch_few(const FewParams& f, hipStream_t stream) {
+  // 32 channels a workgroup where that still gives one to every CU
+  return f.lin.N >= 32 * 256 ? launch_few<2, X>(f, stream) : launch_few<1, X>(f, stream);
+}
 
 template <int TM, int TN, int NB>
 static int launch_linear(LinearParams& p, int workgroups, hipStream_t stream) {
@@ -276,9 +501,9 @@ constexpr int kLinCus = 256;
 
 static int64_t tiles_of(int64_t M, int64_t N, int64_t t) { return ((M + t - 1) / t) * ((N + t - 1) / t); }
 
-extern "C" int qattn_linear_int8(const int8_t* x, int64_t x_pitch, const float* x_scale, const int8_t* w,
-                                 int64_t w_pitch, const float* w_scale, const float* bias, void* out, int out_dtype,
-                                 int64_t out_stride, int64_t M, int64_t N, int64_t K, int act, qattn_stream_t stream) {
+// The checks that both entries share, and the parameters.
+static int linear_params(LinearParams& p, const int8_t* w, int64_t w_pitch, const float* w_scale, const float* bias,
+                         void* out, int out_dtype, int64_t out_stride, int64_t M, int64_t N, int64_t K, int act) {
   QATTN_REQUIRE(out_dtype >= QATTN_BF16 && out_dtype <= QATTN_F32, QATTN_ERR_DTYPE, "linear_int8: out has dtype code %d",
                 out_dtype);
   QATTN_REQUIRE(M >= 0 && N >= 1 && M <= ((int64_t)1 << 31) && N <= (1 << 24), QATTN_ERR_SHAPE,
@@ -287,24 +512,133 @@ extern "C" int qattn_linear_int8(const int8_t* x, int64_t x_pitch, const float* 
                 "linear_int8: K = %lld must be a multiple of 128 up to 131072 (int32 sums)", (long long)K);
   QATTN_REQUIRE(act >= QATTN_ACT_NONE && act <= QATTN_ACT_SILU, QATTN_ERR_ARG, "linear_int8: act code %d", act);
   if (M == 0) return QATTN_OK;
-  QATTN_REQUIRE(x && x_scale && w && w_scale && out, QATTN_ERR_ARG, "linear_int8: a null operand");
-  QATTN_REQUIRE(x_pitch >= K && w_pitch >= K && x_pitch % 16 == 0 && w_pitch % 16 == 0 && x_pitch <= (1 << 22) &&
-                    w_pitch <= (1 << 22),
-                QATTN_ERR_STRIDE, "linear_int8: pitches %lld, %lld must be multiples of 16 from K to 2^22",
-                (long long)x_pitch, (long long)w_pitch);
-  QATTN_REQUIRE(out_stride >= N, QATTN_ERR_STRIDE, "linear_int8: out_stride %lld below N", (long long)out_stride);
-  QATTN_REQUIRE(aligned16(x) && aligned16(w), QATTN_ERR_ALIGN, "linear_int8: x and w must be 16-byte aligned");
-  QATTN_REQUIRE(reinterpret_cast<uintptr_t>(out) % (out_dtype == QATTN_F32 ? 4 : 2) == 0 &&
-                    (reinterpret_cast<uintptr_t>(x_scale) | reinterpret_cast<uintptr_t>(w_scale) |
-                     reinterpret_cast<uintptr_t>(bias)) % 4 == 0,
-                QATTN_ERR_ALIGN, "linear_int8: out, a scale or the bias is misaligned");
   QATTN_REQUIRE(tiles_of(M, N, 128) < ((int64_t)1 << 30), QATTN_ERR_SHAPE, "linear_int8: more than 2^30 tiles");
+  QATTN_REQUIRE(w && w_scale && out, QATTN_ERR_ARG, "linear_int8: a null operand");
+  QATTN_REQUIRE(w_pitch >= K && w_pitch % 16 == 0 && w_pitch <= (1 << 22), QATTN_ERR_STRIDE,
+                "linear_int8: w_pitch %lld must be a multiple of 16 from K to 2^22", (long long)w_pitch);
+  QATTN_REQUIRE(out_stride >= N, QATTN_ERR_STRIDE, "linear_int8: out_stride %lld below N", (long long)out_stride);
+  QATTN_REQUIRE(aligned16(w), QATTN_ERR_ALIGN, "linear_int8: w must be 16-byte aligned");
+  QATTN_REQUIRE(reinterpret_cast<uintptr_t>(out) % (out_dtype == QATTN_F32 ? 4 : 2) == 0 &&
+                    (reinterpret_cast<uintptr_t>(w_scale) | reinterpret_cast<uintptr_t>(bias)) % 4 == 0,
+                QATTN_ERR_ALIGN, "linear_int8: out, a scale or the bias is misaligned");
   const int es = out_dtype == QATTN_F32 ? 4 : 2;
   const bool vec = aligned16(out) && (M == 1 || out_stride * es % 16 == 0);
-  LinearParams p{x, x_pitch, x_scale, w, w_pitch, w_scale, bias, out, out_dtype, vec, out_stride, M, N, (int)K, act, 0, 0};
-  // Rounds of the chip, each tile at its own cost: a stage of the large tile takes 1.2 us (1.6 at the power limit), of the
-  // small one 0.46 (1560 x 1536 x 8960: 85 / 32 us; 512 x 5120 x 4096: 43 / 17)
-  const int64_t large = (tiles_of(M, N, 256) + kLinCus - 1) / kLinCus, small = (tiles_of(M, N, 128) + kLinCus - 1) / kLinCus;
-  if (large * 120 <= small * 46) return launch_linear<256, 256, 2>(p, kLinCus, (hipStream_t)stream);
-  return launch_linear<128, 128, 4>(p, INT32_MAX, (hipStream_t)stream);
+  p = LinearParams{nullptr, 0, nullptr, w, w_pitch, w_scale, bias, out, out_dtype, vec, out_stride, M, N, (int)K, act, 0, 0, nullptr, 0};
+  return QATTN_OK;
+}
+
+// Which kernel, by estimated microseconds (tile kernels: per stage and round of the chip, and 2 to start and end).
+enum LinearKernel { LINEAR_FEW, LINEAR_LARGE, LINEAR_SMALL };
+struct LinearPlan {
+  LinearKernel kernel;
+  int splits, split_stages;
+};
+static LinearPlan plan_linear(int64_t M, int64_t N, int64_t K) {
+  if (M <= kFewRows) return {LINEAR_FEW, 1, 0};
+  // a stage of the large tile takes 1.2 us (1.6 at the power limit), of the small one 0.46 (1560 x 1536 x 8960: 85 / 32
+  // us; 512 x 5120 x 4096: 43 / 17)
+  const int64_t large = tiles_of(M, N, 256), small = tiles_of(M, N, 128), stages = K / kLinK;
+  if ((large + kLinCus - 1) / kLinCus * 120 <= (small + kLinCus - 1) / kLinCus * 46) return {LINEAR_LARGE, 1, 0};
+  auto rounds = [&](int64_t workgroups, int64_t stages) {
+    return (double)((workgroups + kLinCus - 1) / kLinCus) * (0.46 * stages + 2);
+  };
+  LinearPlan best{LINEAR_SMALL, 1, (int)stages};
+  double least = 0.9 * rounds(small, stages);
+  for (int64_t s = 2; s <= 16 && s * small <= 2 * kLinCus && s * 4 <= stages; s++) {
+    // splits write their int32 sums, the join reads them: 5 TB/s, and 3 us for its launch
+    const int64_t per = (stages + s - 1) / s, splits = (stages + per - 1) / per;
+    const double t = rounds(splits * small, per) + 3 + 8.0 * splits * M * N / 5e6;
+    if (t < least) least = t, best = {LINEAR_SMALL, (int)splits, (int)per};
+  }
+  return best;
+}
+static size_t split_bytes(const LinearPlan& plan, int64_t M, int64_t N) {
+  return plan.splits > 1 ? (size_t)plan.splits * tiles_of(M, N, 128) * 128 * 128 * 4 : 0;
+}
+
+static int run_linear(LinearParams& p, const LinearPlan& plan, void* workspace, hipStream_t stream) {
+  if (plan.kernel == LINEAR_FEW) return launch_few<-1>(FewParams{p, nullptr, 0, 0, 1, 0, false}, stream);
+  if (plan.kernel == LINEAR_LARGE) return launch_linear<256, 256, 2>(p, kLinCus, stream);
+  if (plan.splits == 1) return launch_linear<128, 128, 4>(p, INT32_MAX, stream);
+  p.part = static_cast<v4i*>(workspace), p.split_stages = plan.split_stages;
+  p.tiles_m = (int)((p.M + 127) / 128), p.tiles_n = (int)((p.N + 127) / 128);
+  const int tiles = p.tiles_m * p.tiles_n;
+  linear_int8_kernel<128, 128, 4, kSplit><<<dim3((unsigned)(tiles * plan.splits)), dim3(512), 0, stream>>>(p);
+  if (int rc = check_launch("linear_int8")) return rc;
+  const dim3 grid((unsigned)(tiles * 8)), block(256);
+  if (p.act == QATTN_ACT_GELU_TANH) linear_join_kernel<QATTN_ACT_GELU_TANH><<<grid, block, 0, stream>>>(p, plan.splits);
+  else if (p.act == QATTN_ACT_SILU) linear_join_kernel<QATTN_ACT_SILU><<<grid, block, 0, stream>>>(p, plan.splits);
+  else linear_join_kernel<QATTN_ACT_NONE><<<grid, block, 0, stream>>>(p, plan.splits);
+  return check_launch("linear_int8");
+}
+
+static int check_workspace(const void* workspace, size_t bytes, size_t need) {
+  QATTN_REQUIRE(!need || (workspace && bytes >= need && aligned16(workspace)), QATTN_ERR_WORKSPACE,
+                "linear_int8: workspace of %zu bytes, %zu needed (16-byte aligned)", bytes, need);
+  return QATTN_OK;
+}
+
+extern "C" size_t qattn_linear_int8_workspace_size(int64_t M, int64_t N, int64_t K) {
+  return M > 0 && N > 0 && K > 0 ? split_bytes(plan_linear(M, N, K), M, N) : 0;
+}
+
+extern "C" int qattn_linear_int8(const int8_t* x, int64_t x_pitch, const float* x_scale, const int8_t* w,
+                                 int64_t w_pitch, const float* w_scale, const float* bias, void* out, int out_dtype,
+                                 int64_t out_stride, int64_t M, int64_t N, int64_t K, int act, void* workspace,
+                                 size_t workspace_bytes, qattn_stream_t stream) {
+  LinearParams p;
+  if (int rc = linear_params(p, w, w_pitch, w_scale, bias, out, out_dtype, out_stride, M, N, K, act)) return rc;
+  if (M == 0) return QATTN_OK;
+  QATTN_REQUIRE(x && x_scale, QATTN_ERR_ARG, "linear_int8: a null operand");
+  QATTN_REQUIRE(x_pitch >= K && x_pitch % 16 == 0 && x_pitch <= (1 << 22), QATTN_ERR_STRIDE,
+                "linear_int8: x_pitch %lld must be a multiple of 16 from K to 2^22", (long long)x_pitch);
+  QATTN_REQUIRE(aligned16(x) && reinterpret_cast<uintptr_t>(x_scale) % 4 == 0, QATTN_ERR_ALIGN,
+                "linear_int8: x or x_scale is misaligned");
+  p.x = x, p.x_pitch = x_pitch, p.x_scale = x_scale;
+  const LinearPlan plan = plan_linear(M, N, K);
+  if (int rc = check_workspace(workspace, workspace_bytes, split_bytes(plan, M, N))) return rc;
+  return run_linear(p, plan, workspace, (hipStream_t)stream);
+}
+
+static bool few_values(int64_t M, int64_t K) { return M <= kFewRows && M * K <= kFewValues; }
+// the INT8 rows, their scales, and the split sums from a multiple of 16 on
+static size_t rows_bytes(int64_t M, int64_t K) { return (size_t)(M * K + M * 4 + 15) / 16 * 16; }
+
+extern "C" size_t qattn_linear_int8_rows_workspace_size(int64_t M, int64_t N, int64_t cols) {
+  if (M <= 0 || N <= 0 || cols <= 0) return 0;
+  const int64_t K = (cols + 127) / 128 * 128;
+  return few_values(M, K) ? 0 : rows_bytes(M, K) + split_bytes(plan_linear(M, N, K), M, N);
+}
+
+extern "C" int qattn_linear_int8_rows(const void* x, int x_dtype, int64_t x_sb, int64_t x_sl, int64_t B, int64_t L,
+                                      int64_t cols, const int8_t* w, int64_t w_pitch, const float* w_scale,
+                                      const float* bias, void* out, int out_dtype, int64_t out_stride, int64_t N, int act,
+                                      void* workspace, size_t workspace_bytes, qattn_stream_t stream) {
+  QATTN_REQUIRE(x_dtype >= QATTN_BF16 && x_dtype <= QATTN_F32, QATTN_ERR_DTYPE, "linear_int8: x has dtype code %d", x_dtype);
+  QATTN_REQUIRE(cols >= 1 && cols <= 131072 && B >= 0 && L >= 0 && (B == 0 || L <= ((int64_t)1 << 31) / B),
+                QATTN_ERR_SHAPE, "linear_int8: x of %lld x %lld rows of %lld", (long long)B, (long long)L, (long long)cols);
+  const int64_t M = B * L, K = (cols + 127) / 128 * 128;
+  LinearParams p;
+  if (int rc = linear_params(p, w, w_pitch, w_scale, bias, out, out_dtype, out_stride, M, N, K, act)) return rc;
+  if (M == 0) return QATTN_OK;
+  QATTN_REQUIRE(x, QATTN_ERR_ARG, "linear_int8: a null operand");
+  QATTN_REQUIRE(reinterpret_cast<uintptr_t>(x) % (x_dtype == QATTN_F32 ? 4 : 2) == 0, QATTN_ERR_ALIGN,
+                "linear_int8: x is misaligned");
+  if (few_values(M, K)) {
+    const int64_t xs = x_dtype == QATTN_F32 ? 4 : 2, xb = B > 1 ? x_sb : 0, xl = L > 1 ? x_sl : 0;
+    const bool vec = (reinterpret_cast<uintptr_t>(x) | xb * xs | xl * xs) % (4 * xs) == 0;
+    const FewParams f{p, x, xb, xl, (int)L, (int)cols, vec};
+    return x_dtype == QATTN_F32 ? launch_few<QATTN_F32>(f, (hipStream_t)stream)
+           : x_dtype == QATTN_FP16 ? launch_few<QATTN_FP16>(f, (hipStream_t)stream)
+                                   : launch_few<QATTN_BF16>(f, (hipStream_t)stream);
+  }
+  const LinearPlan plan = plan_linear(M, N, K);
+  if (int rc = check_workspace(workspace, workspace_bytes, rows_bytes(M, K) + split_bytes(plan, M, N))) return rc;
+  qattn_block_norm_args q{};
+  q.size = sizeof(q);
+  q.x = x, q.x_dtype = x_dtype, q.x_sb = x_sb, q.x_sl = x_sl, q.B = B, q.L = L, q.C = cols;
+  q.z = workspace, q.z_dtype = QATTN_I8, q.z_pitch = K, q.z_scale = reinterpret_cast<float*>(static_cast<char*>(workspace) + M * K);
+  if (int rc = qattn_block_norm(&q, stream)) return rc;
+  p.x = static_cast<const int8_t*>(workspace), p.x_pitch = K, p.x_scale = q.z_scale;
+  return run_linear(p, plan, static_cast<char*>(workspace) + rows_bytes(M, K), (hipStream_t)stream);
 }

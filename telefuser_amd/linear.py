@@ -12,7 +12,7 @@ from typing import Optional, Union
 import torch
 
 from . import _lib
-from .norm import _DTYPE, Int8Rows, _no_grad, per_token_int8
+from .norm import _DTYPE, Int8Rows, _check_input, _gpu, _no_grad, _rows, per_token_int8
 
 _ACT = {None: 0, "none": 0, "gelu_tanh": 1, "silu": 2}
 _MAX_K = 131072  # 127 * 127 * K stays in int32
@@ -70,36 +70,69 @@ def int8_linear(x: Union[torch.Tensor, Int8Rows], weight: Int8Weight, *, act: Op
     float16 or float32; x's by default, bfloat16 for ``Int8Rows``."""
     if not isinstance(weight, Int8Weight):
         raise ValueError(f"weight must be an Int8Weight, got {type(weight).__name__}")
-    if act not in _ACT:
+    act_code = _ACT.get(act)
+    if act_code is None:
         raise ValueError(f"act must be None, 'gelu_tanh' or 'silu', got {act!r}")
-    if not isinstance(x, Int8Rows):
-        if x.shape[-1:] != (weight.in_features,):
-            raise ValueError(f"x has {tuple(x.shape)}, the weight takes {weight.in_features} channels")
-        out_dtype = out_dtype or x.dtype
-        x = per_token_int8(x)
-    out_dtype = out_dtype or torch.bfloat16
-    if out_dtype not in _DTYPE:
+    lib, n, w, bias = _lib.load(), weight.out_features, weight.codes, weight.bias
+    kpad = w.shape[1]
+    if isinstance(x, Int8Rows):
+        return _linear_rows(lib, x, weight, act_code, out_dtype)
+    x_dt = _check_input(x, "x")
+    shape = x.shape
+    if shape[-1] != weight.in_features:
+        raise ValueError(f"x has {tuple(shape)}, the weight takes {weight.in_features} channels")
+    _no_grad(x)
+    dev = _gpu(x)
+    if w.get_device() != dev:
+        raise ValueError(f"x is on {x.device}, the weight on {w.device}")
+    out_dtype = out_dtype or x.dtype
+    out_dt = _out_code(out_dtype)
+    out = x.new_empty((*shape[:-1], n), dtype=out_dtype)
+    B, L = 1 if len(shape) == 2 else shape[0], shape[-2]
+    if B and L:
+        xr, sb, sl = _rows(x)
+        size = lib.qattn_linear_int8_rows_workspace_size(B * L, n, shape[-1])
+        ws = x.new_empty(size, dtype=torch.uint8) if size else None
+        with _lib.on_device(dev):
+            _lib.check(lib.qattn_linear_int8_rows(
+                xr.data_ptr(), x_dt, sb, sl, B, L, shape[-1], w.data_ptr(), kpad, weight.scale.data_ptr(),
+                None if bias is None else bias.data_ptr(), out.data_ptr(), out_dt, n, n, act_code,
+                None if ws is None else ws.data_ptr(), size, _lib.raw_stream(dev)))
+    return out
+
+
+def _out_code(out_dtype: torch.dtype) -> int:
+    code = _DTYPE.get(out_dtype)
+    if code is None:
         raise ValueError(f"out_dtype must be bfloat16, float16 or float32, got {out_dtype}")
-    codes, x_scale = x.codes, x.scale
-    kpad = weight.codes.shape[1]
-    if x.cols != weight.in_features or codes.shape[-1] != kpad:
-        raise ValueError(f"x has {x.cols} channels in rows of {codes.shape[-1]}, the weight takes {weight.in_features} "
+    return code
+
+
+def _linear_rows(lib, x: Int8Rows, weight: Int8Weight, act_code: int, out_dtype):
+    codes, x_scale, cols = x
+    out_dtype = out_dtype or torch.bfloat16
+    out_dt = _out_code(out_dtype)
+    kpad, n = weight.codes.shape[1], weight.out_features
+    if cols != weight.in_features or codes.shape[-1] != kpad:
+        raise ValueError(f"x has {cols} channels in rows of {codes.shape[-1]}, the weight takes {weight.in_features} "
                          f"in rows of {kpad}")
-    dev = codes.device
+    dev = codes.get_device()
     if codes.dtype != torch.int8 or x_scale.dtype != torch.float32 or codes.shape[:-1] != x_scale.shape or \
-            not codes.is_contiguous() or not x_scale.is_contiguous() or x_scale.device != dev:
+            not codes.is_contiguous() or not x_scale.is_contiguous() or x_scale.get_device() != dev:
         raise ValueError("Int8Rows must hold contiguous int8 codes and a contiguous float32 scale for each row")
-    if dev.type != "cuda" or weight.codes.device != dev:
-        raise ValueError(f"x is on {dev}, the weight on {weight.codes.device}: both must be on one GPU")
-    n = weight.out_features
-    out = torch.empty((*codes.shape[:-1], n), dtype=out_dtype, device=dev)
+    if not codes.is_cuda or weight.codes.get_device() != dev:
+        raise ValueError(f"x is on {codes.device}, the weight on {weight.codes.device}: both must be on one GPU")
+    out = codes.new_empty((*codes.shape[:-1], n), dtype=out_dtype)
     m = x_scale.numel()
     if m:
+        bias = weight.bias
+        size = lib.qattn_linear_int8_workspace_size(m, n, kpad)
+        ws = codes.new_empty(size) if size else None
         with _lib.on_device(dev):
-            _lib.check(_lib.load().qattn_linear_int8(
+            _lib.check(lib.qattn_linear_int8(
                 codes.data_ptr(), kpad, x_scale.data_ptr(), weight.codes.data_ptr(), kpad, weight.scale.data_ptr(),
-                None if weight.bias is None else weight.bias.data_ptr(), out.data_ptr(), _DTYPE[out_dtype], n, m, n,
-                kpad, _ACT[act], _lib.stream_of(codes)))
+                None if bias is None else bias.data_ptr(), out.data_ptr(), out_dt, n, m, n, kpad, act_code,
+                None if ws is None else ws.data_ptr(), size, _lib.raw_stream(dev)))
     return out
 
 

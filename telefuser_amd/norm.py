@@ -24,6 +24,7 @@ from . import _lib
 _NORM = {None: 0, "layer": 1, "rms": 2}
 _DTYPE = {torch.bfloat16: _lib.QATTN_BF16, torch.float16: _lib.QATTN_FP16, torch.float32: _lib.QATTN_F32}
 _NO_PARAM = _lib.QattnParam(None, 0, 0, 0)
+_ARGS_SIZE = ctypes.sizeof(_lib.QattnBlockNormArgs)
 
 
 class Int8Rows(NamedTuple):
@@ -41,95 +42,112 @@ class Int8Rows(NamedTuple):
 
 
 def _no_grad(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError("no backward: call under torch.no_grad() or detach the inputs")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError("no backward: call under torch.no_grad() or detach the inputs")
 
 
-def _check_input(x: torch.Tensor, name: str) -> None:
-    if x.dtype not in _DTYPE:
+def _check_input(x: torch.Tensor, name: str) -> int:
+    """The dtype code of x after the checks that every input takes."""
+    code = _DTYPE.get(x.dtype)
+    if code is None:
         raise ValueError(f"{name} must be bfloat16, float16 or float32, got {x.dtype}")
-    if x.dim() not in (2, 3):
-        raise ValueError(f"{name} must be [L, C] or [B, L, C], got {tuple(x.shape)}")
-    if x.shape[-1] == 0:
+    shape = x.shape
+    if len(shape) not in (2, 3):
+        raise ValueError(f"{name} must be [L, C] or [B, L, C], got {tuple(shape)}")
+    if shape[-1] == 0:
         raise ValueError(f"{name} has no channels")
+    return code
+
+
+def _gpu(x: torch.Tensor) -> int:
+    if not x.is_cuda:
+        raise ValueError(f"x must be on a GPU, got {x.device}")
+    return x.get_device()
 
 
 def _rows(x: torch.Tensor):
     """x with contiguous channels, and its strides over (b, l)."""
-    if x.stride(-1) != 1 and x.shape[-1] > 1:
+    st = x.stride()
+    if st[-1] != 1 and x.shape[-1] > 1:
         x = x.contiguous()
-    return (x, 0, x.stride(0)) if x.dim() == 2 else (x, x.stride(0), x.stride(1))
+        st = x.stride()
+    return (x, 0, st[0]) if len(st) == 2 else (x, st[0], st[1])
 
 
 def _param(t: Optional[torch.Tensor], x: torch.Tensor, name: str, keep: list):
     """A parameter that broadcasts against x, as the kernels read it; tensors that must outlive the call go to keep."""
     if t is None:
         return _NO_PARAM
-    if t.dtype not in _DTYPE:
+    code = _DTYPE.get(t.dtype)
+    if code is None:
         raise ValueError(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
-    if t.device != x.device:
+    if t.get_device() != x.get_device():
         raise ValueError(f"{name} is on {t.device}, x on {x.device}")
-    shape, c = t.shape, x.shape[-1]
-    if len(shape) > x.dim() or any(n not in (1, m) for n, m in zip(shape[::-1], x.shape[::-1])):
-        raise ValueError(f"{name} {tuple(shape)} does not broadcast against x {tuple(x.shape)}")
-    if c > 1 and (not shape or shape[-1] != c or t.stride(-1) != 1):  # one value for all channels, or strided channels
+    shape, st, like = t.shape, t.stride(), x.shape
+    n, c = len(shape), like[-1]
+    fits = n <= len(like)
+    for i in range(1, min(n, len(like)) + 1):
+        fits = fits and shape[-i] in (1, like[-i])
+    if not fits:
+        raise ValueError(f"{name} {tuple(shape)} does not broadcast against x {tuple(like)}")
+    if c > 1 and (n == 0 or shape[-1] != c or st[-1] != 1):  # one value for all channels, or strided channels
         t = t.expand(*shape[:-1], c).contiguous()
         keep.append(t)
-    n = t.dim()
-    sl = t.stride(-2) if n > 1 and t.shape[-2] > 1 else 0
-    sb = t.stride(0) if n > 2 and t.shape[0] > 1 else 0
-    return _lib.QattnParam(t.data_ptr(), sb, sl, _DTYPE[t.dtype])
+        st = t.stride()
+    sl = st[-2] if n > 1 and shape[-2] > 1 else 0
+    sb = st[0] if n > 2 and shape[0] > 1 else 0
+    return _lib.QattnParam(t.data_ptr(), sb, sl, code)
 
 
 def _run(x, y, gate, residual_scale, post, post_weight, post_bias, post_eps, want_h, norm, weight, bias, scale, shift,
          eps, z_dtype):
-    _check_input(x, "x")
+    x_dt = _check_input(x, "x")
     if norm not in _NORM or post not in _NORM:
         raise ValueError(f"a norm is 'layer' or 'rms', got {norm!r}, {post!r}")
     if not eps >= 0 or not post_eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps}, {post_eps}")
     _no_grad(x, y, gate, post_weight, post_bias, weight, bias, scale, shift)
-    dev = x.device
-    if dev.type != "cuda":
-        raise ValueError(f"x must be on a GPU, got {dev}")
+    dev = _gpu(x)
+    shape = x.shape
     keep = []
     xr, x_sb, x_sl = _rows(x)
     y_ptr = y_sb = y_sl = y_dt = 0
     if y is not None:
-        _check_input(y, "y")
-        if y.shape != x.shape or y.device != dev:
-            raise ValueError(f"y must be {tuple(x.shape)} on {dev}, got {tuple(y.shape)} on {y.device}")
-        if y.dtype != x.dtype and x.dtype != torch.float32:
+        y_dt = _check_input(y, "y")
+        if y.shape != shape or y.get_device() != dev:
+            raise ValueError(f"y must be {tuple(shape)} on {x.device}, got {tuple(y.shape)} on {y.device}")
+        if y_dt != x_dt and x_dt != _lib.QATTN_F32:
             raise ValueError(f"y must have x's dtype {x.dtype} (or x be float32), got {y.dtype}")
         yr, y_sb, y_sl = _rows(y)
         keep.append(yr)
-        y_ptr, y_dt = yr.data_ptr(), _DTYPE[y.dtype]
-    B, (L, C) = (1 if x.dim() == 2 else x.shape[0]), x.shape[-2:]
-    h = z = codes = z_scale = None
-    pitch = 0
+        y_ptr = yr.data_ptr()
+    B, (L, C) = (1 if len(shape) == 2 else shape[0]), shape[-2:]
+    h = z = h_ptr = z_ptr = s_ptr = None
+    pitch = z_dt = 0
     if want_h:
-        h = torch.empty(x.shape, dtype=x.dtype, device=dev)
-    if z_dtype == torch.int8:
-        pitch = -(-C // 128) * 128
-        codes = torch.empty((*x.shape[:-1], pitch), dtype=torch.int8, device=dev)
-        z_scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
-        z = Int8Rows(codes, z_scale, C)
+        h = x.new_empty(shape)
+        h_ptr = h.data_ptr()
+    if z_dtype is torch.int8:
+        pitch, z_dt = -(-C // 128) * 128, _lib.QATTN_I8
+        z = Int8Rows(x.new_empty((*shape[:-1], pitch), dtype=torch.int8), x.new_empty(shape[:-1], dtype=torch.float32), C)
+        z_ptr, s_ptr = z.codes.data_ptr(), z.scale.data_ptr()
     elif z_dtype is not None:
-        if z_dtype not in _DTYPE:
+        z_dt = _DTYPE.get(z_dtype)
+        if z_dt is None:
             raise ValueError(f"out_dtype must be bfloat16, float16, float32 or int8, got {z_dtype}")
-        z = codes = torch.empty(x.shape, dtype=z_dtype, device=dev)
-    params = [_param(t, x, n, keep) for t, n in ((gate, "gate"), (weight, "weight"), (bias, "bias"), (scale, "scale"),
-                                                 (shift, "shift"), (post_weight, "post_weight"),
-                                                 (post_bias, "post_bias"))]
+        z = x.new_empty(shape, dtype=z_dtype)
+        z_ptr = z.data_ptr()
     if B and L:
         args = _lib.QattnBlockNormArgs(
-            ctypes.sizeof(_lib.QattnBlockNormArgs), xr.data_ptr(), y_ptr, h.data_ptr() if want_h else None,
-            codes.data_ptr() if codes is not None else None, z_scale.data_ptr() if z_scale is not None else None, x_sb,
-            x_sl, y_sb, y_sl, pitch, B, L, C, *params, _DTYPE[x.dtype], y_dt,
-            _lib.QATTN_I8 if z_scale is not None else _DTYPE.get(z_dtype, 0), _NORM[norm], _NORM[post], eps, post_eps,
-            residual_scale)
+            _ARGS_SIZE, xr.data_ptr(), y_ptr, h_ptr, z_ptr, s_ptr, x_sb, x_sl, y_sb, y_sl, pitch, B, L, C,
+            _param(gate, x, "gate", keep), _param(weight, x, "weight", keep), _param(bias, x, "bias", keep),
+            _param(scale, x, "scale", keep), _param(shift, x, "shift", keep),
+            _param(post_weight, x, "post_weight", keep), _param(post_bias, x, "post_bias", keep), x_dt, y_dt, z_dt,
+            _NORM[norm], _NORM[post], eps, post_eps, residual_scale)
         with _lib.on_device(dev):
-            _lib.check(_lib.load().qattn_block_norm(args, _lib.stream_of(x)))
+            _lib.check(_lib.load().qattn_block_norm(args, _lib.raw_stream(dev)))
     return h, z
 
 

@@ -139,10 +139,10 @@ def test_empty_calls_launch_nothing(lib):
 
 
 def _linear(lib, **kw):
-    a = dict(x=4096, xp=128, sx=4096, w=4096, wp=128, sw=4096, bias=None, out=4096, dt=0, os=64, M=2, N=64, K=128, act=0)
+    a = dict(x=4096, xp=128, sx=4096, w=4096, wp=128, sw=4096, bias=None, out=4096, dt=0, os=64, M=2, N=64, K=128, act=0, ws=None, wb=0)
     a.update(kw)
     return lib.qattn_linear_int8(a["x"], a["xp"], a["sx"], a["w"], a["wp"], a["sw"], a["bias"], a["out"], a["dt"], a["os"],
-                                 a["M"], a["N"], a["K"], a["act"], None)
+                                 a["M"], a["N"], a["K"], a["act"], a["ws"], a["wb"], None)
 
 
 @pytest.mark.parametrize("kw,code", [
@@ -150,7 +150,34 @@ def _linear(lib, **kw):
     ({"K": 131200, "xp": 131200, "wp": 131200}, 2), ({"act": 3}, 9), ({"act": -1}, 9), ({"x": None}, 9), ({"sx": None}, 9),
     ({"w": None}, 9), ({"sw": None}, 9), ({"out": None}, 9), ({"xp": 64}, 3), ({"wp": 136}, 3), ({"os": 63}, 3),
     ({"x": 4104}, 4), ({"w": 4097}, 4), ({"out": 4097}, 4), ({"out": 4098, "dt": 2}, 4), ({"sw": 4098}, 4),
-    ({"bias": 4098}, 4), ({"xp": 1 << 23}, 3),
+    ({"bias": 4098}, 4), ({"xp": 1 << 23}, 3), ({"M": 64, "K": 8192, "xp": 8192, "wp": 8192}, 7),
+    ({"M": 64, "K": 8192, "xp": 8192, "wp": 8192, "ws": 4104, "wb": 1 << 30}, 7),
+    ({"M": 64, "K": 8192, "xp": 8192, "wp": 8192, "ws": 4096, "wb": 2 * 128 * 128 * 4 - 1}, 7),
 ])
 def test_linear_status(lib, kw, code):
     assert _linear(lib, **kw) == code, lib.qattn_last_error()
+
+
+@pytest.mark.parametrize("kw,code", [
+    ({"xd": 3}, 1), ({"cols": 0}, 2), ({"cols": 131073}, 2), ({"B": -1}, 2), ({"L": 1 << 40}, 2), ({"x": None}, 9),
+    ({"x": 4097}, 4), ({"w": None}, 9), ({"wp": 128}, 3), ({"os": 63}, 3), ({"act": 7}, 9), ({"ws": None}, 7),
+    ({"wb": 99 * 260 + 3}, 7), ({"ws": 4104}, 7), ({"dt": 9}, 1),
+])
+def test_linear_rows_status(lib, kw, code):
+    a = dict(x=4096, xd=0, B=1, L=99, cols=200, w=4096, wp=256, out=4096, dt=0, os=64, N=64, act=0, ws=4096, wb=99 * 260 + 4)
+    a.update(kw)
+    rc = lib.qattn_linear_int8_rows(a["x"], a["xd"], 0, 200, a["B"], a["L"], a["cols"], a["w"], a["wp"], 4096, None,
+                                    a["out"], a["dt"], a["os"], a["N"], a["act"], a["ws"], a["wb"], None)
+    assert rc == code, lib.qattn_last_error()
+
+
+def test_linear_workspaces(lib):
+    rows, split = lib.qattn_linear_int8_rows_workspace_size, lib.qattn_linear_int8_workspace_size
+    assert rows(0, 64, 100) == rows(5, 0, 100) == rows(5, 64, 0) == rows(1, 64, 16384) == rows(16, 64, 1024) == 0
+    assert rows(1, 64, 16385) == 16528 and rows(99, 64, 200) == 99 * 260 + 4 and rows(75600, 64, 5120) == 75600 * 5124
+    # split along K: few tiles and many stages, whole tiles of int32 sums
+    assert split(75600, 13824, 5120) == split(1560, 1536, 8960) == split(200, 64, 256) == split(16, 64, 8960) == 0
+    for m, n, k in ((17, 100, 4096), (64, 1536, 8960), (100, 9216, 13824)):
+        tiles = -(-m // 128) * -(-n // 128)
+        assert split(m, n, k) % (tiles * 128 * 128 * 4) == 0 and 2 <= split(m, n, k) // (tiles * 128 * 128 * 4) <= 16
+        assert rows(m, n, k) == (m * k + m * 4 + 15) // 16 * 16 + split(m, n, k)

@@ -128,6 +128,29 @@ def test_shapes_strides_and_quantized_weights():
     assert torch.equal(strided.codes, weight.codes)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("B,L,K", [(1, 1, 1), (1, 1, 16384), (1, 16, 1024), (2, 8, 1000), (4, 4, 1024), (3, 5, 130),
+                                   (1, 7, 2049), (5, 1, 3200), (1, 17, 100), (1, 9, 1920)])
+def test_few_tokens_quantized_on_the_way(B, L, K, dtype):
+    """A floating x of few values (and just more than a few) gives the bits of its INT8 rows, whatever its strides."""
+    require_gpu()
+    from telefuser_amd.linear import Int8Weight, int8_linear
+    from telefuser_amd.norm import per_token_int8
+
+    weight = Int8Weight(*_weight(100, K, 2))
+    big = _x((B + 1, L + 2, K + 9), K, dtype)
+    big[0, 0, 0] = float("inf")
+    for v in (big[1:, :L, :K], big[1:, 1:L + 1, 3:K + 3], big[1:, 2:, 8:K + 8].clone(), big.transpose(0, 1)[1:L + 1, 1:, :K]):
+        for act in (None, "silu"):
+            assert torch.equal(int8_linear(v, weight, act=act), int8_linear(per_token_int8(v), weight, act=act,
+                                                                            out_dtype=dtype))
+    zero = torch.zeros((B, L, K), dtype=dtype, device="cuda")
+    zero[0, 0, K // 2] = float("nan")
+    out = int8_linear(zero, weight, out_dtype=FP32)
+    assert torch.isnan(out[0, 0]).all()
+    assert torch.equal(out.reshape(B * L, -1)[1:], weight.bias.expand(B * L - 1, -1))
+
+
 def test_offsets_past_32_bits():
     require_gpu()
     from telefuser_amd.linear import Int8Rows, Int8Weight, int8_linear
