@@ -9,6 +9,14 @@
 //
 // Everything between the loads and the stores is fp32; v reaches the norm unrounded.  The variance is that of the
 // centred values.  Parameters are read with the strides of their broadcast shape.
+//
+// Bound by memory: x (and y) read once, h and z written once.  At the rate of a copy (5.1 TB/s for 1 GiB) or above where
+// the caches help: gated residual + norm of 75600 x 5120 bf16 0.58 ms (5.3 TB/s), norm of it 306 us (5.1), norm of
+// 32760 x 1536 34 us, row quantizer of 75600 x 5120 206 us (5.6).  What it took: every value loaded once and held in
+// registers (8.4 ms with the row read again for each reduction); reductions over DPP instead of LDS; 16-byte accesses at any
+// alignment (20000 x 5119, one element a load: 405 us, now 130); several narrow rows a wave (75600 x 64: 25 us, now 7);
+// parameters in LDS for many rows; and few VALU instructions a value, which INT8 output has most of: masks only in groups
+// that the row's end cuts, one fused multiply-add for a code of a normalized value (20000 x 5120 to INT8: 110 us, now 88).
 #include "attn_device.h"
 
 namespace qattn {
@@ -34,6 +42,7 @@ struct BlockNormParams {
   int64_t L, rows;
   int C, norm, post_norm;
   float eps, post_eps, residual_scale;
+  int staged[5], stage_half;  // offsets in LDS of the staged parameters (floats), or -1; floats of a half
 };
 
 __device__ __forceinline__ float load_elem(const void* p, int dtype, int64_t i) {
@@ -52,79 +61,73 @@ __device__ __forceinline__ float load_param(const Param& q, int64_t b, int64_t l
 // ------------------------------------------------------------------------------------------------
 // rows held in registers
 // ------------------------------------------------------------------------------------------------
-// A workgroup of W waves takes a row, every thread NV groups of 8 channels: each value is loaded once, the reductions
-// run over registers (DPP within a wave, LDS between waves), and the outputs are written from them.
-//   VEC:  groups of 8 consecutive channels in 16-byte loads (32 for fp32); everything divides by 8 and is aligned.
-//   else: channel (8 i + e) T + tid, one element per load: any width, stride and alignment.
-constexpr int kRowGroup = 8;
-constexpr int kMaxRowWaves = 8;
-
+// A thread holds NV groups of 8 consecutive channels of a row: every value is loaded once, the reductions run over
+// registers, and the outputs are written from them.  A group is one 16-byte access (two for fp32) at whatever alignment
+// its row has; only a group that the row's end cuts goes element by element.
 enum YMode { Y_NONE, Y_SAME, Y_BF16, Y_FP16 };
 
-template <int DT, bool VEC>
+typedef v4u v4u_any __attribute__((aligned(2)));  // rows of halves start anywhere
+typedef v4u v4u_word __attribute__((aligned(4)));
+
+template <int DT>
 struct RawGroup {
-  static constexpr int kWords = DT == QATTN_F32 ? 8 : VEC ? 4 : 8;  // scalar halves: one word each
+  static constexpr int kWords = DT == QATTN_F32 ? 8 : 4;
   uint32_t w[kWords];
-  __device__ __forceinline__ void load(const void* p, int64_t at, int c, int step, int C) {
-    if constexpr (VEC) {
-      if (c < C) {
-        constexpr int kSize = DT == QATTN_F32 ? 4 : 2;
-        const v4u* q = reinterpret_cast<const v4u*>(static_cast<const char*>(p) + (at + c) * kSize);
+  // channels c .. c + 7 of the row at `at` of `C` channels, zeros past its end; whole: known to lie within
+  __device__ __forceinline__ void load(const void* p, int64_t at, int c, int C, bool whole) {
+    if (whole || c + 8 <= C) {
+      if constexpr (DT == QATTN_F32) {
+        const v4u_word* q = reinterpret_cast<const v4u_word*>(static_cast<const float*>(p) + at + c);
+        const v4u a = q[0], b = q[1];
 #pragma unroll
-        for (int k = 0; k < kWords / 4; k++) {
-          const v4u v = q[k];
-#pragma unroll
-          for (int e = 0; e < 4; e++) w[4 * k + e] = v[e];
-        }
+        for (int e = 0; e < 4; e++) w[e] = a[e], w[4 + e] = b[e];
       } else {
+        const v4u a = *reinterpret_cast<const v4u_any*>(static_cast<const uint16_t*>(p) + at + c);
 #pragma unroll
-        for (int e = 0; e < kWords; e++) w[e] = 0;
+        for (int e = 0; e < 4; e++) w[e] = a[e];
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const int cc = c + e * step;
-        if constexpr (DT == QATTN_F32) w[e] = cc < C ? static_cast<const uint32_t*>(p)[at + cc] : 0u;
-        else w[e] = cc < C ? static_cast<const uint16_t*>(p)[at + cc] : 0u;
-      }
+      for (int e = 0; e < kWords; e++) w[e] = 0;
+#pragma unroll
+      for (int e = 0; e < 7; e++)
+        if (c + e < C) {
+          if constexpr (DT == QATTN_F32) w[e] = static_cast<const uint32_t*>(p)[at + c + e];
+          else w[e / 2] |= (uint32_t)static_cast<const uint16_t*>(p)[at + c + e] << (16 * (e & 1));
+        }
     }
   }
   __device__ __forceinline__ float get(int e) const {
     if constexpr (DT == QATTN_F32) return __uint_as_float(w[e]);
-    const uint16_t h = VEC ? (uint16_t)(w[e / 2] >> (16 * (e & 1))) : (uint16_t)w[e];
-    return half_to_f32<DT == QATTN_FP16>(h);
+    else return half_to_f32<DT == QATTN_FP16>((uint16_t)(w[e / 2] >> (16 * (e & 1))));
   }
 };
 
-template <bool VEC>
-__device__ __forceinline__ void load_param8(const Param& q, int64_t b, int64_t l, int c, int step, int C, float (&out)[8]) {
-  const int64_t at = b * q.sb + l * q.sl;
+__device__ __forceinline__ void load_param8(const Param& q, int64_t at, int c, int C, bool whole, float (&out)[8]) {
   if (q.dtype == QATTN_F32) {
-    RawGroup<QATTN_F32, VEC> g;
-    g.load(q.p, at, c, step, C);
+    RawGroup<QATTN_F32> g;
+    g.load(q.p, at, c, C, whole);
 #pragma unroll
     for (int e = 0; e < 8; e++) out[e] = g.get(e);
   } else {
-    RawGroup<QATTN_BF16, VEC> g;
-    g.load(q.p, at, c, step, C);
+    RawGroup<QATTN_BF16> g;
+    g.load(q.p, at, c, C, whole);
     if (q.dtype == QATTN_BF16) {
 #pragma unroll
       for (int e = 0; e < 8; e++) out[e] = g.get(e);
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; e++) out[e] = f16_to_f32(VEC ? (uint16_t)(g.w[e / 2] >> (16 * (e & 1))) : (uint16_t)g.w[e]);
+      for (int e = 0; e < 8; e++) out[e] = f16_to_f32((uint16_t)(g.w[e / 2] >> (16 * (e & 1))));
     }
   }
 }
 
-template <bool VEC>
-__device__ __forceinline__ void store8(void* p, int dtype, int64_t at, int c, int step, int C, const float (&v)[8]) {
-  if constexpr (VEC) {
-    if (c >= C) return;
+__device__ __forceinline__ void store8(void* p, int dtype, int64_t at, int c, int C, bool whole, const float (&v)[8]) {
+  if (whole || c + 8 <= C) {
     if (dtype == QATTN_F32) {
-      v4f* q = reinterpret_cast<v4f*>(static_cast<float*>(p) + at + c);
-      q[0] = v4f{v[0], v[1], v[2], v[3]};
-      q[1] = v4f{v[4], v[5], v[6], v[7]};
+      v4u_word* q = reinterpret_cast<v4u_word*>(static_cast<float*>(p) + at + c);
+      q[0] = v4u{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+      q[1] = v4u{__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])};
     } else {
       v4u o;
       if (dtype == QATTN_FP16) {
@@ -134,145 +137,220 @@ __device__ __forceinline__ void store8(void* p, int dtype, int64_t at, int c, in
 #pragma unroll
         for (int e = 0; e < 4; e++) o[e] = pack_half2<false>(v[2 * e], v[2 * e + 1]);
       }
-      *reinterpret_cast<v4u*>(static_cast<uint16_t*>(p) + at + c) = o;
+      *reinterpret_cast<v4u_any*>(static_cast<uint16_t*>(p) + at + c) = o;
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; e++)
-      if (c + e * step < C) store_elem(p, dtype, at + c + e * step, v[e]);
+    for (int e = 0; e < 7; e++)
+      if (c + e < C) store_elem(p, dtype, at + c + e, v[e]);
   }
 }
 
-// Reductions over the workgroup; each call has its own LDS slots, so one barrier separates write and read.
+// Reductions over the lanes of a row: LANES of a wave, or whole waves (each call then has its own LDS slots, so one
+// barrier separates write and read).
+constexpr int kMaxRowWaves = 8;
+template <int LANES>
 struct RowReduce {
   uint32_t (*slots)[kMaxRowWaves];
   int waves, wave;
   int used = 0;
+  template <typename OP>
+  __device__ __forceinline__ uint32_t reduce(uint32_t v, OP op) {
+    if constexpr (LANES < 64) {
+      v = op(v, dpp<0xb1, 0xf>(0u, v));
+      v = op(v, dpp<0x4e, 0xf>(0u, v));
+      v = op(v, dpp<0x141, 0xf>(0u, v));
+      if constexpr (LANES > 8) v = op(v, dpp<0x140, 0xf>(0u, v));
+      if constexpr (LANES > 16) v = op(v, (uint32_t)__shfl_xor((int)v, 16, 64));
+      return v;
+    } else {
+      uint32_t t = wave_reduce(v, 0u, op);
+      if (waves == 1) return t;
+      uint32_t* s = slots[used++];
+      if ((threadIdx.x & 63) == 0) s[wave] = t;
+      __syncthreads();
+      t = s[0];
+      for (int i = 1; i < waves; i++) t = op(t, s[i]);
+      return t;
+    }
+  }
   __device__ __forceinline__ float sum(float v) {
-    float t = wave_total(v);
-    if (waves == 1) return t;
-    uint32_t* s = slots[used++];
-    if ((threadIdx.x & 63) == 0) s[wave] = __float_as_uint(t);
-    __syncthreads();
-    t = 0.0f;
-    for (int i = 0; i < waves; i++) t += __uint_as_float(s[i]);
-    return t;
+    return __uint_as_float(reduce(__float_as_uint(v), [](uint32_t a, uint32_t b) {
+      return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+    }));
   }
   __device__ __forceinline__ uint32_t top(uint32_t v) {
-    uint32_t t = wave_top(v);
-    if (waves == 1) return t;
-    uint32_t* s = slots[used++];
-    if ((threadIdx.x & 63) == 0) s[wave] = t;
-    __syncthreads();
-    for (int i = 0; i < waves; i++) t = max(t, s[i]);
-    return t;
+    return reduce(v, [](uint32_t a, uint32_t b) { return max(a, b); });
   }
 };
 
-template <int XD, int YM, bool VEC, int NV>
-__global__ __launch_bounds__(kMaxRowWaves * 64) void row_norm_kernel(BlockNormParams p) {
-  constexpr int YD = YM == Y_BF16 ? QATTN_BF16 : YM == Y_FP16 ? QATTN_FP16 : XD;
-  __shared__ uint32_t slots[5][kMaxRowWaves];
-  const int T = blockDim.x, tid = threadIdx.x, step = VEC ? 1 : T;
-  RowReduce red{slots, T >> 6, tid >> 6};
-  const int64_t row = blockIdx.x;
-  const int64_t b = row / p.L, l = row - b * p.L;
-  const int C = p.C;
-  const float inv_c = 1.0f / (float)C;
-  auto first = [&](int i) { return VEC ? (i * T + tid) * 8 : i * 8 * T + tid; };
-  // out-of-row values of the scalar form: element e of group i is beyond the row
-  auto in_row = [&](int i, int e) { return first(i) + (VEC ? 0 : e * T) < C; };
-
-  RawGroup<XD, VEC> xr[NV];
-  RawGroup<YD, VEC> yr[YM == Y_NONE ? 1 : NV];
-  const int64_t xo = b * p.xb + l * p.xl, yo = b * p.yb + l * p.yl;
+// Where a row's parameters come from: memory, with the strides of their broadcast shape, ...
+struct DirectParams {
+  const BlockNormParams& p;
+  int64_t b, l;
+  __device__ __forceinline__ void load(const Param& q, int c, bool whole, float (&t)[8]) const {
+    load_param8(q, b * q.sb + l * q.sl, c, p.C, whole, t);
+  }
+  __device__ __forceinline__ bool post(int c, bool whole, float (&mul)[8], float (&add)[8]) const {
 #pragma unroll
-  for (int i = 0; i < NV; i++) xr[i].load(p.x, xo, first(i), step, C);
-  if constexpr (YM != Y_NONE)
+    for (int e = 0; e < 8; e++) mul[e] = 1.0f, add[e] = 0.0f;
+    if (p.post_weight.p) load(p.post_weight, c, whole, mul);
+    if (p.post_bias.p) load(p.post_bias, c, whole, add);
+    return p.post_weight.p || p.post_bias.p;
+  }
+  __device__ __forceinline__ bool gate(int c, bool whole, float (&t)[8]) const {
+    if (p.gate.p) load(p.gate, c, whole, t);
+    return p.gate.p;
+  }
+  // weight, bias, scale and shift as one multiplication and one addition
+  __device__ __forceinline__ bool affine(int c, bool whole, float (&mul)[8], float (&add)[8]) const {
 #pragma unroll
-    for (int i = 0; i < NV; i++) yr[i].load(p.y, yo, first(i), step, C);
-
-  float v[NV][8];
-  if constexpr (YM != Y_NONE) {
+    for (int e = 0; e < 8; e++) mul[e] = 1.0f, add[e] = 0.0f;
+    if (p.weight.p) load(p.weight, c, whole, mul);
+    if (p.bias.p) load(p.bias, c, whole, add);
+    if (p.scale.p) {
+      float t[8];
+      load(p.scale, c, whole, t);
 #pragma unroll
-    for (int i = 0; i < NV; i++)
-#pragma unroll
-      for (int e = 0; e < 8; e++) v[i][e] = yr[i].get(e);
-    if (p.post_norm) {
-      float mean = 0.0f, s = 0.0f;
-      if (p.post_norm == QATTN_NORM_LAYER) {
-#pragma unroll
-        for (int i = 0; i < NV; i++)
-#pragma unroll
-          for (int e = 0; e < 8; e++) s += v[i][e];
-        mean = red.sum(s) * inv_c;
-        s = 0.0f;
-      }
-#pragma unroll
-      for (int i = 0; i < NV; i++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          v[i][e] = in_row(i, e) ? v[i][e] - mean : 0.0f;
-          s = fmaf(v[i][e], v[i][e], s);
-        }
-      const float rstd = 1.0f / sqrtf(red.sum(s) * inv_c + p.post_eps);
-#pragma unroll
-      for (int i = 0; i < NV; i++) {
-        float t[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) v[i][e] *= rstd;
-        if (p.post_weight.p) {
-          load_param8<VEC>(p.post_weight, b, l, first(i), step, C, t);
-#pragma unroll
-          for (int e = 0; e < 8; e++) v[i][e] *= t[e];
-        }
-        if (p.post_bias.p) {
-          load_param8<VEC>(p.post_bias, b, l, first(i), step, C, t);
-#pragma unroll
-          for (int e = 0; e < 8; e++) v[i][e] += t[e];
-        }
-      }
+      for (int e = 0; e < 8; e++) mul[e] = fmaf(mul[e], t[e], mul[e]), add[e] = fmaf(add[e], t[e], add[e]);
     }
+    if (p.shift.p) {
+      float t[8];
+      load(p.shift, c, whole, t);
+#pragma unroll
+      for (int e = 0; e < 8; e++) add[e] += t[e];
+    }
+    return p.weight.p || p.bias.p || p.scale.p || p.shift.p;
+  }
+};
+
+// ... or LDS, where the workgroup has put them once for all of its rows: those that there are of [post mul, post add, gate,
+// mul, add], each as the first halves of all 8-channel groups and then the second ones, so that a wave reads 16 bytes a
+// lane side by side.
+struct StagedParams {
+  const BlockNormParams& p;
+  const float* lds;
+  __device__ __forceinline__ void load(int which, int c, float (&t)[8]) const {
+    // (a thread past the row's end takes the last group's, and drops what it makes of them)
+    const float* q = lds + p.staged[which] + min(c / 2, p.stage_half - 4);
+    const v4f a = *reinterpret_cast<const v4f*>(q), b = *reinterpret_cast<const v4f*>(q + p.stage_half);
+#pragma unroll
+    for (int e = 0; e < 4; e++) t[e] = a[e], t[4 + e] = b[e];
+  }
+  __device__ __forceinline__ bool post(int c, bool, float (&mul)[8], float (&add)[8]) const {
+    if (p.staged[0] < 0) return false;
+    load(0, c, mul), load(1, c, add);
+    return true;
+  }
+  __device__ __forceinline__ bool gate(int c, bool, float (&t)[8]) const {
+    if (p.staged[2] < 0) return false;
+    load(2, c, t);
+    return true;
+  }
+  __device__ __forceinline__ bool affine(int c, bool, float (&mul)[8], float (&add)[8]) const {
+    if (p.staged[3] < 0) return false;
+    load(3, c, mul), load(4, c, add);
+    return true;
+  }
+};
+
+// One row; `first` is the thread's first channel, `step` the distance between its groups.  A group i of which no thread's
+// lies past the row's end (a condition on scalars) takes no masks.
+template <int XD, int YM, int NV>
+struct RowValues {
+  static constexpr int YD = YM == Y_BF16 ? QATTN_BF16 : YM == Y_FP16 ? QATTN_FP16 : XD;
+  RawGroup<XD> x[NV];
+  RawGroup<YD> y[YM == Y_NONE ? 1 : NV];
+  __device__ __forceinline__ void load(const BlockNormParams& p, int64_t b, int64_t l, int first, int step) {
+    const int64_t xo = b * p.xb + l * p.xl, yo = b * p.yb + l * p.yl;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-      if (p.gate.p) {
-        float t[8];
-        load_param8<VEC>(p.gate, b, l, first(i), step, C, t);
-#pragma unroll
-        for (int e = 0; e < 8; e++) v[i][e] *= t[e];
-      }
-#pragma unroll
-      for (int e = 0; e < 8; e++) v[i][e] = fmaf(p.residual_scale, xr[i].get(e), v[i][e]);
+      const bool whole = (i + 1) * step <= p.C;
+      x[i].load(p.x, xo, first + i * step, p.C, whole);
+      if constexpr (YM != Y_NONE) y[i].load(p.y, yo, first + i * step, p.C, whole);
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < NV; i++)
-#pragma unroll
-      for (int e = 0; e < 8; e++) v[i][e] = xr[i].get(e);
   }
-  if (p.h)
-#pragma unroll
-    for (int i = 0; i < NV; i++) store8<VEC>(p.h, XD, row * C, first(i), step, C, v[i]);
-  if (!p.z) return;
+};
 
-  if (p.norm) {
+// r: the row's values, loaded; next() is called once they are used and may load others into r.
+template <int XD, int YM, int NV, typename REDUCE, typename PARAMS, typename NEXT>
+__device__ __forceinline__ void norm_row(const BlockNormParams& p, int64_t b, int64_t l, int first, int step, REDUCE red,
+                                         const PARAMS& params, const RowValues<XD, YM, NV>& r, NEXT next) {
+  const int C = p.C;
+  const int64_t row = b * p.L + l;
+  const float inv_c = 1.0f / (float)C;
+  auto whole = [&](int i) __attribute__((always_inline)) { return (i + 1) * step <= C; };
+  float v[NV][8];
+  // v - mean (or v) in place and 1 / sqrt(var + eps); values past the row's end are zeros before and after
+  auto normalize = [&](int kind, float eps) __attribute__((always_inline)) {
     float mean = 0.0f, s = 0.0f;
-    if (p.norm == QATTN_NORM_LAYER) {
+    if (kind == QATTN_NORM_LAYER) {
 #pragma unroll
       for (int i = 0; i < NV; i++)
 #pragma unroll
         for (int e = 0; e < 8; e++) s += v[i][e];
       mean = red.sum(s) * inv_c;
       s = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[i][e] -= mean;
+        if (!whole(i)) {
+          const int left = C - first - i * step;
+#pragma unroll
+          for (int e = 0; e < 8; e++)
+            if (e >= left) v[i][e] = 0.0f;
+        }
+      }
     }
 #pragma unroll
     for (int i = 0; i < NV; i++)
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        v[i][e] = in_row(i, e) ? v[i][e] - mean : 0.0f;
-        s = fmaf(v[i][e], v[i][e], s);
+      for (int e = 0; e < 8; e++) s = fmaf(v[i][e], v[i][e], s);
+    return 1.0f / sqrtf(red.sum(s) * inv_c + eps);
+  };
+  if constexpr (YM != Y_NONE) {
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[i][e] = r.y[i].get(e);
+    if (p.post_norm) {
+      const float rstd = normalize(p.post_norm, p.post_eps);
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        float mul[8], add[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[i][e] *= rstd;
+        if (params.post(first + i * step, whole(i), mul, add)) {
+          const int left = whole(i) ? 8 : C - first - i * step;  // past the row's end stay zeros: the next norm sums them
+#pragma unroll
+          for (int e = 0; e < 8; e++) v[i][e] = e < left ? fmaf(v[i][e], mul[e], add[e]) : 0.0f;
+        }
       }
-    const float rstd = 1.0f / sqrtf(red.sum(s) * inv_c + p.eps);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      float t[8];
+      if (params.gate(first + i * step, whole(i), t))
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[i][e] *= t[e];
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[i][e] = fmaf(p.residual_scale, r.x[i].get(e), v[i][e]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) v[i][e] = r.x[i].get(e);
+  }
+  next();
+  if (p.h)
+#pragma unroll
+    for (int i = 0; i < NV; i++) store8(p.h, XD, row * C, first + i * step, C, whole(i), v[i]);
+  if (!p.z) return;
+
+  if (p.norm) {
+    const float rstd = normalize(p.norm, p.eps);
 #pragma unroll
     for (int i = 0; i < NV; i++)
 #pragma unroll
@@ -280,57 +358,107 @@ __global__ __launch_bounds__(kMaxRowWaves * 64) void row_norm_kernel(BlockNormPa
   }
 #pragma unroll
   for (int i = 0; i < NV; i++) {
-    float t[8];
-    if (p.weight.p) {
-      load_param8<VEC>(p.weight, b, l, first(i), step, C, t);
+    float mul[8], add[8];
+    if (params.affine(first + i * step, whole(i), mul, add))
 #pragma unroll
-      for (int e = 0; e < 8; e++) v[i][e] *= t[e];
-    }
-    if (p.bias.p) {
-      load_param8<VEC>(p.bias, b, l, first(i), step, C, t);
-#pragma unroll
-      for (int e = 0; e < 8; e++) v[i][e] += t[e];
-    }
-    if (p.scale.p) {
-      load_param8<VEC>(p.scale, b, l, first(i), step, C, t);
-#pragma unroll
-      for (int e = 0; e < 8; e++) v[i][e] = fmaf(v[i][e], t[e], v[i][e]);
-    }
-    if (p.shift.p) {
-      load_param8<VEC>(p.shift, b, l, first(i), step, C, t);
-#pragma unroll
-      for (int e = 0; e < 8; e++) v[i][e] += t[e];
-    }
+      for (int e = 0; e < 8; e++) v[i][e] = fmaf(v[i][e], mul[e], add[e]);
   }
   if (p.z_dtype != QATTN_I8) {
 #pragma unroll
-    for (int i = 0; i < NV; i++) store8<VEC>(p.z, p.z_dtype, row * C, first(i), step, C, v[i]);
+    for (int i = 0; i < NV; i++) store8(p.z, p.z_dtype, row * C, first + i * step, C, whole(i), v[i]);
     return;
   }
   // max|z| as an integer: the bits of |z| are ordered as the values, infinity and NaN above them all
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < NV; i++)
-#pragma unroll
-    for (int e = 0; e < 8; e++)
-      if (in_row(i, e)) top = max(top, __float_as_uint(v[i][e]) & 0x7fffffffu);
-  const RowQuant rq(red.top(top));
-  int8_t* codes = static_cast<int8_t*>(p.z) + row * p.z_pitch;
-#pragma unroll
   for (int i = 0; i < NV; i++) {
-    const int c = first(i);
-    if constexpr (VEC) {
-      if (c < C)
-        *reinterpret_cast<v2u*>(codes + c) = v2u{rq.code4(v[i][0], v[i][1], v[i][2], v[i][3]),
-                                                 rq.code4(v[i][4], v[i][5], v[i][6], v[i][7])};
-    } else {
+    if (!whole(i)) {
+      const int left = C - first - i * step;
 #pragma unroll
       for (int e = 0; e < 8; e++)
-        if (c + e * T < C) codes[c + e * T] = rq.fine ? (int8_t)rq.code(v[i][e]) : (int8_t)0;
+        if (e >= left) v[i][e] = 0.0f;
     }
+#pragma unroll
+    for (int e = 0; e < 8; e += 2)
+      top = max(top, max(__float_as_uint(v[i][e]) & 0x7fffffffu, __float_as_uint(v[i][e + 1]) & 0x7fffffffu));
   }
-  for (int64_t c = C + tid; c < p.z_pitch; c += T) codes[c] = 0;
-  if (tid == 0) p.z_scale[row] = rq.scale;
+  const RowQuant rq(red.top(top));
+  int8_t* codes = static_cast<int8_t*>(p.z) + row * p.z_pitch;
+  // up to the pitch, which divides by 8: the codes past the row's end are those of zeros
+  auto put = [&](auto code4) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+      const int c = first + i * step;
+      if (whole(i) || c < p.z_pitch)
+        *reinterpret_cast<v2u*>(codes + c) = v2u{code4(v[i][0], v[i][1], v[i][2], v[i][3]),
+                                                 code4(v[i][4], v[i][5], v[i][6], v[i][7])};
+    }
+  };
+  if (p.norm) put([&](float a, float b, float c, float d) { return rq.near4(a, b, c, d); });
+  else put([&](float a, float b, float c, float d) { return rq.code4(a, b, c, d); });
+  for (int64_t c = first + NV * step; c < p.z_pitch; c += step) *reinterpret_cast<v2u*>(codes + c) = v2u{0u, 0u};
+  if (first == 0) p.z_scale[row] = rq.scale;
+}
+
+// Narrow rows: LANES lanes a row, several rows a wave.
+template <int XD, int YM, int LANES>
+__global__ __launch_bounds__(256) void narrow_row_kernel(BlockNormParams p) {
+  const int64_t row = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  // a row past the last is the last one again: its lanes take part in the reductions and write what its own lanes write
+  const int64_t at = min(row, p.rows - 1), b = at / p.L, l = at - b * p.L;
+  const int first = threadIdx.x % LANES * 8;
+  RowValues<XD, YM, 1> r;
+  r.load(p, b, l, first, LANES * 8);
+  norm_row<XD, YM, 1>(p, b, l, first, LANES * 8, RowReduce<LANES>{nullptr, 1, 0}, DirectParams{p, b, l}, r, [] {});
+}
+
+// A workgroup a row.
+template <int XD, int YM, int NV>
+__global__ __launch_bounds__(kMaxRowWaves * 64) void row_norm_kernel(BlockNormParams p) {
+  __shared__ uint32_t slots[5][kMaxRowWaves];
+  const int64_t b = blockIdx.x / p.L, l = blockIdx.x - b * p.L;
+  const int first = threadIdx.x * 8, step = blockDim.x * 8;
+  RowValues<XD, YM, NV> r;
+  r.load(p, b, l, first, step);
+  norm_row<XD, YM, NV>(p, b, l, first, step, RowReduce<64>{slots, (int)blockDim.x >> 6, (int)threadIdx.x >> 6},
+                       DirectParams{p, b, l}, r, [] {});
+}
+
+// Many rows with the same parameters: a workgroup folds them and puts them into LDS once, then its eight waves take rows of
+// one batch entry in turn, `waves` of them a row, and load the next row while they work on this one.  Read from memory for
+// every row they are 4 bytes a value and parameter beside the 2 of x, and L2 does not keep up with that.
+template <int XD, int YM, int NV>
+__global__ __launch_bounds__(512) void staged_row_kernel(BlockNormParams p, int waves, int turns) {
+  extern __shared__ __attribute__((aligned(16))) float staged[];
+  __shared__ uint32_t slots[8][2][5][kMaxRowWaves];
+  const int64_t b = blockIdx.y;
+  const DirectParams from{p, b, 0};
+  for (int c = threadIdx.x * 8; c < p.stage_half * 2; c += 512 * 8) {
+    float mul[8], add[8];
+    auto put = [&](int which, const float (&t)[8]) {
+      float* q = staged + p.staged[which] + c / 2;
+      *reinterpret_cast<v4f*>(q) = v4f{t[0], t[1], t[2], t[3]};
+      *reinterpret_cast<v4f*>(q + p.stage_half) = v4f{t[4], t[5], t[6], t[7]};
+    };
+    if (p.staged[0] >= 0) from.post(c, false, mul, add), put(0, mul), put(1, add);
+    if (p.staged[2] >= 0) from.gate(c, false, mul), put(2, mul);
+    if (p.staged[3] >= 0) from.affine(c, false, mul, add), put(3, mul), put(4, add);
+  }
+  __syncthreads();
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), per = 8 / waves, group = wave / waves;
+  const int first = (threadIdx.x - group * waves * 64) * 8, step = waves * 512;
+  // all groups take all turns, for the barriers between a row's waves; past the last row it is the last one again, and gets
+  // the same values
+  auto row = [&](int t) { return min(((int64_t)t * gridDim.x + blockIdx.x) * per + group, p.L - 1); };
+  RowValues<XD, YM, NV> r;
+  r.load(p, b, row(0), first, step);
+  for (int t = 0; t < turns; t++) {
+    // slots alternate: only one barrier may lie between the last read of a row and the next one's write
+    norm_row<XD, YM, NV>(p, b, row(t), first, step, RowReduce<64>{slots[group][t & 1], waves, wave - group * waves},
+                         StagedParams{p, staged}, r, [&] {
+                           if (t + 1 < turns) r.load(p, b, row(t + 1), first, step);
+                         });
+  }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -433,7 +561,7 @@ static int check_param(const qattn_param& q, const char* name, int64_t B, int64_
 static bool row_shape(int C, int& waves, int& groups) {
   const int vecs = (C + 7) / 8;
   int64_t best = -1;
-  for (int nv = 1; nv <= 4; nv++) {
+  for (int nv = 1; nv <= 5; nv++) {
     const int w = (vecs + 64 * nv - 1) / (64 * nv);
     if (w > kMaxRowWaves) continue;
     const int64_t cost = (int64_t)w * nv * 16 + w;
@@ -442,24 +570,59 @@ static bool row_shape(int C, int& waves, int& groups) {
   return best >= 0;
 }
 
-template <int XD, int YM, bool VEC>
-static void launch_rows(const BlockNormParams& p, int waves, int groups, hipStream_t stream) {
-  const dim3 grid((unsigned)p.rows), block(waves * 64);
-  if (groups == 1) row_norm_kernel<XD, YM, VEC, 1><<<grid, block, 0, stream>>>(p);
-  else if (groups == 2) row_norm_kernel<XD, YM, VEC, 2><<<grid, block, 0, stream>>>(p);
-  else if (groups == 3) row_norm_kernel<XD, YM, VEC, 3><<<grid, block, 0, stream>>>(p);
-  else row_norm_kernel<XD, YM, VEC, 4><<<grid, block, 0, stream>>>(p);
-}
-template <int XD, int YM>
-static void launch_rows(const BlockNormParams& p, bool vec, int waves, int groups, hipStream_t stream) {
-  if (vec) launch_rows<XD, YM, true>(p, waves, groups, stream);
-  else launch_rows<XD, YM, false>(p, waves, groups, stream);
+// Staging pays from about this many rows of a batch entry (microseconds, read per row / staged: norm of 9000 x 5120 38.7 /
+// 43.7, of 20000 x 5120 96 / 85, of 75600 x 5120 365 / 306; gated residual + norm of 75600 x 640 111 / 85).
+constexpr int64_t kStagedRows = 16384;
+constexpr int kStagedWidest = 5120;
+// Groups a thread holds in the staged kernel, before a row takes two or four waves.
+constexpr int staged_groups(int dtype) { return dtype == QATTN_F32 ? 3 : 5; }
+constexpr int64_t kCus = 256;
+// Offsets of the folded parameters in LDS, and its bytes; 0 where rows do not share them.
+static size_t stage(BlockNormParams& p, const Param* const* params) {
+  for (int i = 0; i < 7; i++)
+    if (params[i]->p && params[i]->sl) return 0;
+  p.stage_half = (p.C + 7) / 8 * 4;
+  int n = 0;
+  auto take = [&](bool there) { return there ? 2 * p.stage_half * n++ : -1; };
+  const bool post = p.post_norm && (p.post_weight.p || p.post_bias.p);
+  const bool affine = p.z && (p.weight.p || p.bias.p || p.scale.p || p.shift.p);
+  p.staged[0] = take(post), p.staged[1] = take(post);
+  p.staged[2] = take(p.y && p.gate.p);
+  p.staged[3] = take(affine), p.staged[4] = take(affine);
+  return (size_t)n * 2 * p.stage_half * 4;
 }
 
-// every row of 8-channel groups in 16-byte pieces
-static bool vectors(const void* q, int dtype, int64_t sb, int64_t sl) {
-  const int64_t per = 16 / (dtype == QATTN_F32 ? 4 : 2);
-  return aligned16(q) && sb % per == 0 && sl % per == 0;
+template <int XD, int YM>
+static void launch_rows(const BlockNormParams& p, int waves, int groups, size_t lds, hipStream_t stream) {
+  if (lds) {
+    const int vecs = (p.C + 511) / 512, nvmax = staged_groups(XD);
+    const int w = vecs <= nvmax ? 1 : vecs <= 2 * nvmax ? 2 : 4, nv = (vecs + w - 1) / w;
+    // rows of a batch entry in turns, as many workgroups as the CUs hold at once: two to a CU by their registers
+    const int64_t batches = p.rows / p.L, per = 8 / w;
+    const int64_t hold = std::max((int64_t)1, kCus * std::min((int64_t)2, (int64_t)(163840 / (lds + 2560))) / batches);
+    const int64_t turns = (p.L + per * hold - 1) / (per * hold);
+    const dim3 grid((unsigned)((p.L + per * turns - 1) / (per * turns)), (unsigned)batches), block(512);
+    if (nv == 1) staged_row_kernel<XD, YM, 1><<<grid, block, lds, stream>>>(p, w, (int)turns);
+    else if (nv == 2) staged_row_kernel<XD, YM, 2><<<grid, block, lds, stream>>>(p, w, (int)turns);
+    else if (nv == 3) staged_row_kernel<XD, YM, 3><<<grid, block, lds, stream>>>(p, w, (int)turns);
+    else if (nv == 4) staged_row_kernel<XD, YM, 4><<<grid, block, lds, stream>>>(p, w, (int)turns);
+    else staged_row_kernel<XD, YM, 5><<<grid, block, lds, stream>>>(p, w, (int)turns);
+    return;
+  }
+  if (p.C <= 256) {
+    const int lanes = p.C <= 64 ? 8 : p.C <= 128 ? 16 : 32, per = 256 / lanes;
+    const dim3 grid((unsigned)((p.rows + per - 1) / per)), block(256);
+    if (lanes == 8) narrow_row_kernel<XD, YM, 8><<<grid, block, 0, stream>>>(p);
+    else if (lanes == 16) narrow_row_kernel<XD, YM, 16><<<grid, block, 0, stream>>>(p);
+    else narrow_row_kernel<XD, YM, 32><<<grid, block, 0, stream>>>(p);
+    return;
+  }
+  const dim3 grid((unsigned)p.rows), block(waves * 64);
+  if (groups == 1) row_norm_kernel<XD, YM, 1><<<grid, block, 0, stream>>>(p);
+  else if (groups == 2) row_norm_kernel<XD, YM, 2><<<grid, block, 0, stream>>>(p);
+  else if (groups == 3) row_norm_kernel<XD, YM, 3><<<grid, block, 0, stream>>>(p);
+  else if (groups == 4) row_norm_kernel<XD, YM, 4><<<grid, block, 0, stream>>>(p);
+  else row_norm_kernel<XD, YM, 5><<<grid, block, 0, stream>>>(p);
 }
 
 extern "C" int qattn_block_norm(const qattn_block_norm_args* a, qattn_stream_t stream) {
@@ -508,24 +671,26 @@ extern "C" int qattn_block_norm(const qattn_block_norm_args* a, qattn_stream_t s
   p.norm = a->norm, p.post_norm = a->y ? a->post_norm : QATTN_NORM_NONE;
   p.eps = a->eps, p.post_eps = a->post_eps, p.residual_scale = a->residual_scale;
   const hipStream_t st = (hipStream_t)stream;
-  int waves, groups;
-  if (!row_shape(p.C, waves, groups)) {
+  int waves = 1, groups;
+  const bool wide = !row_shape(p.C, waves, groups);
+  QATTN_REQUIRE(p.rows * waves <= ((int64_t)1 << 25), QATTN_ERR_SHAPE,
+                "block_norm: %lld rows of %d channels are more than one launch takes", (long long)p.rows, p.C);
+  if (wide) {
     wide_row_kernel<<<dim3((unsigned)((p.rows + 3) / 4)), 256, 0, st>>>(p);
     return check_launch("block_norm");
   }
-  bool vec = p.C % 8 == 0 && vectors(p.x, p.x_dtype, p.xb, p.xl) && (!p.y || vectors(p.y, p.y_dtype, p.yb, p.yl));
-  for (int i = 0; i < 7; i++) vec = vec && vectors(to[i]->p, to[i]->dtype, to[i]->sb, to[i]->sl);
+  const size_t lds = p.C > 256 && p.C <= kStagedWidest && p.L >= kStagedRows && a->B < 65536 ? stage(p, to) : 0;
   if (p.x_dtype == QATTN_F32) {
-    if (!p.y) launch_rows<QATTN_F32, Y_NONE>(p, vec, waves, groups, st);
-    else if (p.y_dtype == QATTN_F32) launch_rows<QATTN_F32, Y_SAME>(p, vec, waves, groups, st);
-    else if (p.y_dtype == QATTN_BF16) launch_rows<QATTN_F32, Y_BF16>(p, vec, waves, groups, st);
-    else launch_rows<QATTN_F32, Y_FP16>(p, vec, waves, groups, st);
+    if (!p.y) launch_rows<QATTN_F32, Y_NONE>(p, waves, groups, lds, st);
+    else if (p.y_dtype == QATTN_F32) launch_rows<QATTN_F32, Y_SAME>(p, waves, groups, lds, st);
+    else if (p.y_dtype == QATTN_BF16) launch_rows<QATTN_F32, Y_BF16>(p, waves, groups, lds, st);
+    else launch_rows<QATTN_F32, Y_FP16>(p, waves, groups, lds, st);
   } else if (p.x_dtype == QATTN_BF16) {
-    if (p.y) launch_rows<QATTN_BF16, Y_SAME>(p, vec, waves, groups, st);
-    else launch_rows<QATTN_BF16, Y_NONE>(p, vec, waves, groups, st);
+    if (p.y) launch_rows<QATTN_BF16, Y_SAME>(p, waves, groups, lds, st);
+    else launch_rows<QATTN_BF16, Y_NONE>(p, waves, groups, lds, st);
   } else {
-    if (p.y) launch_rows<QATTN_FP16, Y_SAME>(p, vec, waves, groups, st);
-    else launch_rows<QATTN_FP16, Y_NONE>(p, vec, waves, groups, st);
+    if (p.y) launch_rows<QATTN_FP16, Y_SAME>(p, waves, groups, lds, st);
+    else launch_rows<QATTN_FP16, Y_NONE>(p, waves, groups, lds, st);
   }
   return check_launch("block_norm");
 }

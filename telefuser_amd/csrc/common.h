@@ -154,11 +154,19 @@ struct RowQuant {
     const float q = n * rcp;
     return __float_as_uint(fmaf(fmaf(-top, q, n), rcp, q) + 12582912.0f);
   }
+  // x times 127 / max|x| rounded to float32: for values that carry a float32 rounding of their own, which moves a code
+  // across a border as often
+  __device__ __forceinline__ uint32_t near(float x) const { return __float_as_uint(fmaf(x, mult * rcp, 12582912.0f)); }
   // four codes, the first in the low byte
+  __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) const {
+    const uint32_t lo = __builtin_amdgcn_perm(b, a, 0x0c0c0400u), hi = __builtin_amdgcn_perm(d, c, 0x04000c0cu);
+    return fine ? lo | hi : 0u;
+  }
   __device__ __forceinline__ uint32_t code4(float a, float b, float c, float d) const {
-    const uint32_t lo = __builtin_amdgcn_perm(code(b), code(a), 0x0c0c0400u);
-    const uint32_t hi = __builtin_amdgcn_perm(code(d), code(c), 0x0c0c0400u);
-    return fine ? lo | hi << 16 : 0u;
+    return pack4(code(a), code(b), code(c), code(d));
+  }
+  __device__ __forceinline__ uint32_t near4(float a, float b, float c, float d) const {
+    return pack4(near(a), near(b), near(c), near(d));
   }
 };
 

@@ -512,7 +512,7 @@ static int linear_params(LinearParams& p, const int8_t* w, int64_t w_pitch, cons
                 "linear_int8: K = %lld must be a multiple of 128 up to 131072 (int32 sums)", (long long)K);
   QATTN_REQUIRE(act >= QATTN_ACT_NONE && act <= QATTN_ACT_SILU, QATTN_ERR_ARG, "linear_int8: act code %d", act);
   if (M == 0) return QATTN_OK;
-  QATTN_REQUIRE(tiles_of(M, N, 128) < ((int64_t)1 << 30), QATTN_ERR_SHAPE, "linear_int8: more than 2^30 tiles");
+  QATTN_REQUIRE(tiles_of(M, N, 128) < ((int64_t)1 << 23), QATTN_ERR_SHAPE, "linear_int8: more than 2^23 tiles");
   QATTN_REQUIRE(w && w_scale && out, QATTN_ERR_ARG, "linear_int8: a null operand");
   QATTN_REQUIRE(w_pitch >= K && w_pitch % 16 == 0 && w_pitch <= (1 << 22), QATTN_ERR_STRIDE,
                 "linear_int8: w_pitch %lld must be a multiple of 16 from K to 2^22", (long long)w_pitch);

@@ -221,6 +221,39 @@ def test_empty_and_many_rows():
     P.check(block_norm(x), ref, err, "many rows")
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
+@pytest.mark.parametrize("B,L,C", [(1, 16384, 260), (2, 16400, 520), (1, 20011, 1027), (1, 16390, 1536), (1, 17000, 2565),
+                                   (1, 16384, 4097), (2, 16387, 5120)])
+def test_many_rows_of_shared_parameters(B, L, C, dtype):
+    """Long sequences with the parameters of a batch entry: rows from all over, and none written twice or left out."""
+    require_gpu()
+    from telefuser_amd.norm import block_norm, gated_residual, gated_residual_norm
+
+    x, y = _x((B, L, C), C, dtype), _x((B, L, C), C + 1, dtype)
+    at = torch.cat([torch.arange(0, 20), torch.randint(20, L - 20, (60,), generator=torch.Generator().manual_seed(C)),
+                    torch.arange(L - 20, L)]).cuda()
+    xs, ys = x[:, at], y[:, at]
+    gate, scale, shift, w, b, pw = (_p(s, i) for i, s in enumerate([(B, 1, C), (B, 1, C), (1, 1, C), (C,), (C,), (C,)]))
+    for how in ({"scale": scale, "shift": shift}, {"weight": w, "norm": "rms"},
+                {"weight": w, "bias": b, "scale": scale, "shift": shift}):
+        ref = {**how, "norm_kind": how.get("norm", "layer")}
+        ref.pop("norm", None)
+        _, _, rz, ez = P.block(xs, **ref)
+        P.check(block_norm(x, **how)[:, at], rz, ez, f"z {sorted(how)}")
+        rows = block_norm(x, **how, out_dtype=torch.int8)
+        P.check_rows(type(rows)(rows.codes[:, at], rows.scale[:, at], C), rz, ez, f"int8 {sorted(how)}")
+    for how in ({}, {"post_norm": "rms", "post_weight": pw}, {"post_norm": "layer", "post_weight": pw, "post_bias": b}):
+        h, z = gated_residual_norm(x, y, gate, scale=scale, shift=shift, **how)
+        rh, eh, rz, ez = P.block(xs, ys, gate, scale=scale, shift=shift, **how)
+        P.check(h[:, at], rh, eh, f"h {sorted(how)}")
+        P.check(z[:, at], rz, ez, f"z {sorted(how)}")
+        assert torch.equal(gated_residual(x, y, gate, **how), h)
+    full = block_norm(x, scale=scale, shift=shift)  # every row, against the same rows in short calls
+    for i in range(0, L, 8000):
+        part = block_norm(x[:, i:i + 8000], scale=scale, shift=shift)
+        assert ((full[:, i:i + 8000].float() - part.float()).abs() <= 0.02 * (part.float().abs() + 1)).all()
+
+
 def test_offsets_past_32_bits():
     require_gpu()
     from telefuser_amd.norm import gated_residual_norm
