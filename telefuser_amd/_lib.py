@@ -7,7 +7,6 @@ raises, so the HIP kernels are always what runs.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 
@@ -247,16 +246,12 @@ def stream_of(t: torch.Tensor):
 
 
 
-def raw_stream(index: int) -> int:
-    """The handle of the current stream of GPU ``index`` (stream_of without building a Stream object)."""
-    return torch._C._cuda_getCurrentRawStream(index)
-
-
-_HERE_DEVICE = contextlib.nullcontext()
-
-
-def on_device(index: int):
-    """Context in which a launch on a stream of GPU ``index`` is valid: it is made current, unless it is already."""
+def launch(index: int, entry, *args) -> None:
+    """entry(*args, stream) on the current stream of GPU ``index``, which is made the current one for it."""
     if index == torch._C._cuda_getDevice():
-        return _HERE_DEVICE
-    return torch.cuda.device(index)
+        rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc)

@@ -557,11 +557,13 @@ static int check_param(const qattn_param& q, const char* name, int64_t B, int64_
 }
 
 // Waves per row and 8-channel groups per thread: the pair that leaves the fewest lanes idle, of equal ones the one with
-// fewer waves (a reduction between waves takes a barrier).
-static bool row_shape(int C, int& waves, int& groups) {
+// fewer waves (a reduction between waves takes a barrier).  A thread that has only x to read takes up to 5 groups, one that
+// reads y or parameters beside it 2 where 8 waves suffice: its registers then leave room for more waves (2 x 4680 x 5120,
+// 5 / 2 groups at most: row quantizer 25.5 / 31.4 us, norm with per-token scale and shift 113 / 108).
+static bool row_shape(int C, bool plain, int& waves, int& groups) {
   const int vecs = (C + 7) / 8;
   int64_t best = -1;
-  for (int nv = 1; nv <= 5; nv++) {
+  for (int nv = 1; nv <= (plain || best < 0 ? 5 : 2); nv++) {
     const int w = (vecs + 64 * nv - 1) / (64 * nv);
     if (w > kMaxRowWaves) continue;
     const int64_t cost = (int64_t)w * nv * 16 + w;
@@ -672,7 +674,9 @@ extern "C" int qattn_block_norm(const qattn_block_norm_args* a, qattn_stream_t s
   p.eps = a->eps, p.post_eps = a->post_eps, p.residual_scale = a->residual_scale;
   const hipStream_t st = (hipStream_t)stream;
   int waves = 1, groups;
-  const bool wide = !row_shape(p.C, waves, groups);
+  bool plain = !p.y;
+  for (int i = 0; i < 7; i++) plain = plain && !to[i]->p;
+  const bool wide = !row_shape(p.C, plain, waves, groups);
   QATTN_REQUIRE(p.rows * waves <= ((int64_t)1 << 25), QATTN_ERR_SHAPE,
                 "block_norm: %lld rows of %d channels are more than one launch takes", (long long)p.rows, p.C);
   if (wide) {

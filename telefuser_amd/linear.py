@@ -93,11 +93,9 @@ def int8_linear(x: Union[torch.Tensor, Int8Rows], weight: Int8Weight, *, act: Op
         xr, sb, sl = _rows(x)
         size = lib.qattn_linear_int8_rows_workspace_size(B * L, n, shape[-1])
         ws = x.new_empty(size, dtype=torch.uint8) if size else None
-        with _lib.on_device(dev):
-            _lib.check(lib.qattn_linear_int8_rows(
-                xr.data_ptr(), x_dt, sb, sl, B, L, shape[-1], w.data_ptr(), kpad, weight.scale.data_ptr(),
-                None if bias is None else bias.data_ptr(), out.data_ptr(), out_dt, n, n, act_code,
-                None if ws is None else ws.data_ptr(), size, _lib.raw_stream(dev)))
+        _lib.launch(dev, lib.qattn_linear_int8_rows, xr.data_ptr(), x_dt, sb, sl, B, L, shape[-1], w.data_ptr(), kpad,
+                    weight.scale.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), out_dt, n, n,
+                    act_code, None if ws is None else ws.data_ptr(), size)
     return out
 
 
@@ -128,11 +126,9 @@ def _linear_rows(lib, x: Int8Rows, weight: Int8Weight, act_code: int, out_dtype)
         bias = weight.bias
         size = lib.qattn_linear_int8_workspace_size(m, n, kpad)
         ws = codes.new_empty(size) if size else None
-        with _lib.on_device(dev):
-            _lib.check(lib.qattn_linear_int8(
-                codes.data_ptr(), kpad, x_scale.data_ptr(), weight.codes.data_ptr(), kpad, weight.scale.data_ptr(),
-                None if bias is None else bias.data_ptr(), out.data_ptr(), out_dt, n, m, n, kpad, act_code,
-                None if ws is None else ws.data_ptr(), size, _lib.raw_stream(dev)))
+        _lib.launch(dev, lib.qattn_linear_int8, codes.data_ptr(), kpad, x_scale.data_ptr(), weight.codes.data_ptr(), kpad,
+                    weight.scale.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(), out_dt, n, m, n,
+                    kpad, act_code, None if ws is None else ws.data_ptr(), size)
     return out
 
 

@@ -24,6 +24,7 @@ from . import _lib
 _NORM = {None: 0, "layer": 1, "rms": 2}
 _DTYPE = {torch.bfloat16: _lib.QATTN_BF16, torch.float16: _lib.QATTN_FP16, torch.float32: _lib.QATTN_F32}
 _NO_PARAM = _lib.QattnParam(None, 0, 0, 0)
+_PARAMS = ("gate", "weight", "bias", "scale", "shift", "post_weight", "post_bias")
 _ARGS_SIZE = ctypes.sizeof(_lib.QattnBlockNormArgs)
 
 
@@ -87,11 +88,13 @@ def _param(t: Optional[torch.Tensor], x: torch.Tensor, name: str, keep: list):
         raise ValueError(f"{name} is on {t.device}, x on {x.device}")
     shape, st, like = t.shape, t.stride(), x.shape
     n, c = len(shape), like[-1]
-    fits = n <= len(like)
-    for i in range(1, min(n, len(like)) + 1):
-        fits = fits and shape[-i] in (1, like[-i])
-    if not fits:
-        raise ValueError(f"{name} {tuple(shape)} does not broadcast against x {tuple(like)}")
+    if shape != like:
+        fits = n <= len(like)
+        for size, want in zip(shape[::-1], like[::-1]):
+            if size != want and size != 1:
+                fits = False
+        if not fits:
+            raise ValueError(f"{name} {tuple(shape)} does not broadcast against x {tuple(like)}")
     if c > 1 and (n == 0 or shape[-1] != c or st[-1] != 1):  # one value for all channels, or strided channels
         t = t.expand(*shape[:-1], c).contiguous()
         keep.append(t)
@@ -142,12 +145,10 @@ def _run(x, y, gate, residual_scale, post, post_weight, post_bias, post_eps, wan
     if B and L:
         args = _lib.QattnBlockNormArgs(
             _ARGS_SIZE, xr.data_ptr(), y_ptr, h_ptr, z_ptr, s_ptr, x_sb, x_sl, y_sb, y_sl, pitch, B, L, C,
-            _param(gate, x, "gate", keep), _param(weight, x, "weight", keep), _param(bias, x, "bias", keep),
-            _param(scale, x, "scale", keep), _param(shift, x, "shift", keep),
-            _param(post_weight, x, "post_weight", keep), _param(post_bias, x, "post_bias", keep), x_dt, y_dt, z_dt,
+            *[_NO_PARAM if t is None else _param(t, x, name, keep) for name, t in zip(_PARAMS, (
+                gate, weight, bias, scale, shift, post_weight, post_bias))], x_dt, y_dt, z_dt,
             _NORM[norm], _NORM[post], eps, post_eps, residual_scale)
-        with _lib.on_device(dev):
-            _lib.check(_lib.load().qattn_block_norm(args, _lib.raw_stream(dev)))
+        _lib.launch(dev, _lib.load().qattn_block_norm, args)
     return h, z
 
 
