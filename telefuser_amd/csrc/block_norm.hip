@@ -556,30 +556,33 @@ static int check_param(const qattn_param& q, const char* name, int64_t B, int64_
   return QATTN_OK;
 }
 
-// Waves per row and 8-channel groups per thread: the pair that leaves the fewest lanes idle, of equal ones the one with
-// fewer waves (a reduction between waves takes a barrier).  A thread that has only x to read takes up to 5 groups, one that
-// reads y or parameters beside it 2 where 8 waves suffice: its registers then leave room for more waves (2 x 4680 x 5120,
-// 5 / 2 groups at most: row quantizer 25.5 / 31.4 us, norm with per-token scale and shift 113 / 108).
+// Waves per row and 8-channel groups per thread, by the groups of 8 lanes that they occupy (idle ones too) and by the
+// waves.  A thread that has only x to read takes up to 5 groups, and a wave more costs as much as 12 lanes' worth of groups:
+// reductions between waves take barriers (row quantizer of 39606 x 3328 with 7 / 4 / 3 / 2 waves: 134 / 99 / 96 / 79 us).
+// One that reads y or parameters beside it takes 2 where 8 waves suffice: its registers then leave room for more waves
+// (2 x 4680 x 5120, 5 / 2 groups at most: norm with per-token scale and shift 113 / 108 us).
 static bool row_shape(int C, bool plain, int& waves, int& groups) {
   const int vecs = (C + 7) / 8;
   int64_t best = -1;
   for (int nv = 1; nv <= (plain || best < 0 ? 5 : 2); nv++) {
     const int w = (vecs + 64 * nv - 1) / (64 * nv);
     if (w > kMaxRowWaves) continue;
-    const int64_t cost = (int64_t)w * nv * 16 + w;
+    const int64_t cost = (int64_t)w * nv * 16 + w * (plain ? 24 : 1);
     if (best < 0 || cost < best) best = cost, waves = w, groups = nv;
   }
   return best >= 0;
 }
 
 // Staging pays from about this many rows of a batch entry (microseconds, read per row / staged: norm of 9000 x 5120 38.7 /
-// 43.7, of 20000 x 5120 96 / 85, of 75600 x 5120 365 / 306; gated residual + norm of 75600 x 640 111 / 85).
+// 43.7, of 20000 x 5120 96 / 85, of 75600 x 5120 365 / 306; gated residual + norm of 75600 x 640 111 / 85, of 48306 x 7040 685 / 516).
 constexpr int64_t kStagedRows = 16384;
-constexpr int kStagedWidest = 5120;
+constexpr int kStagedWidest = 8192;
+constexpr size_t kLds = 163840, kSlotBytes = 8 * 2 * 5 * kMaxRowWaves * 4;
 // Groups a thread holds in the staged kernel, before a row takes two or four waves.
 constexpr int staged_groups(int dtype) { return dtype == QATTN_F32 ? 3 : 5; }
 constexpr int64_t kCus = 256;
-// Offsets of the folded parameters in LDS, and its bytes; 0 where rows do not share them.
+// Offsets of the folded parameters in LDS, and its bytes; 0 where rows do not share them or LDS does not hold
+// them.
 static size_t stage(BlockNormParams& p, const Param* const* params) {
   for (int i = 0; i < 7; i++)
     if (params[i]->p && params[i]->sl) return 0;
@@ -591,7 +594,8 @@ static size_t stage(BlockNormParams& p, const Param* const* params) {
   p.staged[0] = take(post), p.staged[1] = take(post);
   p.staged[2] = take(p.y && p.gate.p);
   p.staged[3] = take(affine), p.staged[4] = take(affine);
-  return (size_t)n * 2 * p.stage_half * 4;
+  const size_t bytes = (size_t)n * 2 * p.stage_half * 4;
+  return bytes + kSlotBytes <= kLds ? bytes : 0;
 }
 
 template <int XD, int YM>
@@ -601,7 +605,7 @@ static void launch_rows(const BlockNormParams& p, int waves, int groups, size_t 
     const int w = vecs <= nvmax ? 1 : vecs <= 2 * nvmax ? 2 : 4, nv = (vecs + w - 1) / w;
     // rows of a batch entry in turns, as many workgroups as the CUs hold at once: two to a CU by their registers
     const int64_t batches = p.rows / p.L, per = 8 / w;
-    const int64_t hold = std::max((int64_t)1, kCus * std::min((int64_t)2, (int64_t)(163840 / (lds + 2560))) / batches);
+    const int64_t hold = std::max((int64_t)1, kCus * std::min((int64_t)2, (int64_t)(kLds / (lds + kSlotBytes))) / batches);
     const int64_t turns = (p.L + per * hold - 1) / (per * hold);
     const dim3 grid((unsigned)((p.L + per * turns - 1) / (per * turns)), (unsigned)batches), block(512);
     if (nv == 1) staged_row_kernel<XD, YM, 1><<<grid, block, lds, stream>>>(p, w, (int)turns);

@@ -223,7 +223,7 @@ def test_empty_and_many_rows():
 
 @pytest.mark.parametrize("dtype", [BF16, FP16, FP32])
 @pytest.mark.parametrize("B,L,C", [(1, 16384, 260), (2, 16400, 520), (1, 20011, 1027), (1, 16390, 1536), (1, 17000, 2565),
-                                   (1, 16384, 4097), (2, 16387, 5120)])
+                                   (1, 16384, 4097), (2, 16387, 5120), (1, 16400, 8192)])
 def test_many_rows_of_shared_parameters(B, L, C, dtype):
     """Long sequences with the parameters of a batch entry: rows from all over, and none written twice or left out."""
     require_gpu()
@@ -247,7 +247,8 @@ def test_many_rows_of_shared_parameters(B, L, C, dtype):
         rh, eh, rz, ez = P.block(xs, ys, gate, scale=scale, shift=shift, **how)
         P.check(h[:, at], rh, eh, f"h {sorted(how)}")
         P.check(z[:, at], rz, ez, f"z {sorted(how)}")
-        assert torch.equal(gated_residual(x, y, gate, **how), h)
+        # (not the bits of h: without the norm's parameters another kernel may run, which sums a row in another order)
+        P.check(gated_residual(x, y, gate, **how)[:, at], rh, eh, f"h alone {sorted(how)}")
     full = block_norm(x, scale=scale, shift=shift)  # every row, against the same rows in short calls
     for i in range(0, L, 8000):
         part = block_norm(x[:, i:i + 8000], scale=scale, shift=shift)
