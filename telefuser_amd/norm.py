@@ -14,7 +14,6 @@ Forward only, like the attention they surround: inputs that need a gradient are 
 
 from __future__ import annotations
 
-import ctypes
 from typing import NamedTuple, Optional
 
 import torch
@@ -23,9 +22,8 @@ from . import _lib
 
 _NORM = {None: 0, "layer": 1, "rms": 2}
 _DTYPE = {torch.bfloat16: _lib.QATTN_BF16, torch.float16: _lib.QATTN_FP16, torch.float32: _lib.QATTN_F32}
-_NO_PARAM = _lib.QattnParam(None, 0, 0, 0)
-_PARAMS = ("gate", "weight", "bias", "scale", "shift", "post_weight", "post_bias")
-_ARGS_SIZE = ctypes.sizeof(_lib.QattnBlockNormArgs)
+_NO_PARAM = (0, 0, 0, 0)
+_pack_args, _ARGS_SIZE = _lib.BLOCK_NORM_ARGS.pack, _lib.BLOCK_NORM_ARGS.size
 
 
 class Int8Rows(NamedTuple):
@@ -77,10 +75,9 @@ def _rows(x: torch.Tensor):
     return (x, 0, st[0]) if len(st) == 2 else (x, st[0], st[1])
 
 
-def _param(t: Optional[torch.Tensor], x: torch.Tensor, name: str, keep: list):
-    """A parameter that broadcasts against x, as the kernels read it; tensors that must outlive the call go to keep."""
-    if t is None:
-        return _NO_PARAM
+def _param(t: torch.Tensor, x: torch.Tensor, name: str, keep: list):
+    """A parameter that broadcasts against x, as the fields of qattn_param; tensors that must outlive the call go to
+    keep."""
     code = _DTYPE.get(t.dtype)
     if code is None:
         raise ValueError(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
@@ -101,7 +98,7 @@ def _param(t: Optional[torch.Tensor], x: torch.Tensor, name: str, keep: list):
         st = t.stride()
     sl = st[-2] if n > 1 and shape[-2] > 1 else 0
     sb = st[0] if n > 2 and shape[0] > 1 else 0
-    return _lib.QattnParam(t.data_ptr(), sb, sl, code)
+    return t.data_ptr(), sb, sl, code
 
 
 def _run(x, y, gate, residual_scale, post, post_weight, post_bias, post_eps, want_h, norm, weight, bias, scale, shift,
@@ -127,10 +124,10 @@ def _run(x, y, gate, residual_scale, post, post_weight, post_bias, post_eps, wan
         keep.append(yr)
         y_ptr = yr.data_ptr()
     B, (L, C) = (1 if len(shape) == 2 else shape[0]), shape[-2:]
-    h = z = h_ptr = z_ptr = s_ptr = None
-    pitch = z_dt = 0
+    h = z = None
+    h_ptr = z_ptr = s_ptr = pitch = z_dt = 0
     if want_h:
-        h = x.new_empty(shape)
+        h = torch.empty_like(x, memory_format=torch.contiguous_format)
         h_ptr = h.data_ptr()
     if z_dtype is torch.int8:
         pitch, z_dt = -(-C // 128) * 128, _lib.QATTN_I8
@@ -140,14 +137,19 @@ def _run(x, y, gate, residual_scale, post, post_weight, post_bias, post_eps, wan
         z_dt = _DTYPE.get(z_dtype)
         if z_dt is None:
             raise ValueError(f"out_dtype must be bfloat16, float16, float32 or int8, got {z_dtype}")
-        z = x.new_empty(shape, dtype=z_dtype)
+        z = torch.empty_like(x, dtype=z_dtype, memory_format=torch.contiguous_format)
         z_ptr = z.data_ptr()
     if B and L:
-        args = _lib.QattnBlockNormArgs(
+        args = _pack_args(
             _ARGS_SIZE, xr.data_ptr(), y_ptr, h_ptr, z_ptr, s_ptr, x_sb, x_sl, y_sb, y_sl, pitch, B, L, C,
-            *[_NO_PARAM if t is None else _param(t, x, name, keep) for name, t in zip(_PARAMS, (
-                gate, weight, bias, scale, shift, post_weight, post_bias))], x_dt, y_dt, z_dt,
-            _NORM[norm], _NORM[post], eps, post_eps, residual_scale)
+            *(_NO_PARAM if gate is None else _param(gate, x, "gate", keep)),
+            *(_NO_PARAM if weight is None else _param(weight, x, "weight", keep)),
+            *(_NO_PARAM if bias is None else _param(bias, x, "bias", keep)),
+            *(_NO_PARAM if scale is None else _param(scale, x, "scale", keep)),
+            *(_NO_PARAM if shift is None else _param(shift, x, "shift", keep)),
+            *(_NO_PARAM if post_weight is None else _param(post_weight, x, "post_weight", keep)),
+            *(_NO_PARAM if post_bias is None else _param(post_bias, x, "post_bias", keep)),
+            x_dt, y_dt, z_dt, _NORM[norm], _NORM[post], eps, post_eps, residual_scale)
         _lib.launch(dev, _lib.load().qattn_block_norm, args)
     return h, z
 

@@ -89,8 +89,8 @@ def test_parameter_strides():
 
     def strides(t):
         keep = []
-        q = norm._param(t, X, "gate", keep)
-        return q.sb, q.sl, len(keep)
+        _, sb, sl, _ = norm._param(t, X, "gate", keep)
+        return sb, sl, len(keep)
 
     assert strides(torch.ones(64)) == (0, 0, 0)
     assert strides(torch.ones(3, 64)) == (0, 64, 0)
@@ -116,7 +116,20 @@ def _norm_args(**kw):
                                 64, none, none, none, none, none, none, none, 0, 0, 0, 1, 0, 1e-6, 0.0, 1.0)
     for k, v in kw.items():
         setattr(a, k, v)
-    return a
+    return ctypes.byref(a)
+
+
+def test_packed_args_are_the_struct():
+    a = _lib.QattnBlockNormArgs
+    assert _lib.BLOCK_NORM_ARGS.size == ctypes.sizeof(a)
+    param = (11, 12, 13, 2)
+    values = (1, 2, 3, 4, 5, 6, *range(21, 29), *param * 7, 31, 32, 33, 34, 35, 0.5, 0.25, 2.0)
+    got = a.from_buffer_copy(_lib.BLOCK_NORM_ARGS.pack(*values))
+    flat = []
+    for name, kind in a._fields_:
+        v = getattr(got, name)
+        flat += [getattr(v, n) for n, _ in kind._fields_] if kind is _lib.QattnParam else [v]
+    assert tuple(flat) == values
 
 
 @pytest.mark.parametrize("kw,code", [
