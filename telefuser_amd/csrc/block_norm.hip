@@ -394,7 +394,7 @@ __device__ __forceinline__ void norm_row(const BlockNormParams& p, int64_t b, in
                                                  code4(v[i][4], v[i][5], v[i][6], v[i][7])};
     }
   };
-  if (p.norm) put([&](float a, float b, float c, float d) { return rq.near4(a, b, c, d); });
+  if (p.norm && rq.nearable()) put([&](float a, float b, float c, float d) { return rq.near4(a, b, c, d); });
   else put([&](float a, float b, float c, float d) { return rq.code4(a, b, c, d); });
   for (int64_t c = first + NV * step; c < p.z_pitch; c += step) *reinterpret_cast<v2u*>(codes + c) = v2u{0u, 0u};
   if (first == 0) p.z_scale[row] = rq.scale;

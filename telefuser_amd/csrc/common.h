@@ -155,7 +155,8 @@ struct RowQuant {
     return __float_as_uint(fmaf(fmaf(-top, q, n), rcp, q) + 12582912.0f);
   }
   // x times 127 / max|x| rounded to float32: for values that carry a float32 rounding of their own, which moves a code
-  // across a border as often
+  // across a border as often; where max|x| is not scaled up (127 / max|x| would not be finite)
+  __device__ __forceinline__ bool nearable() const { return mult <= 127.0f; }
   __device__ __forceinline__ uint32_t near(float x) const { return __float_as_uint(fmaf(x, mult * rcp, 12582912.0f)); }
   // four codes, the first in the low byte
   __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) const {

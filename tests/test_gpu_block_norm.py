@@ -193,6 +193,26 @@ def test_int8_rows_of_extreme_values(K):
     assert rows.scale[0] == 0 and torch.isnan(rows.scale[1:]).all()
 
 
+@pytest.mark.parametrize("C", [40, 200, 1536])
+@pytest.mark.parametrize("w", [1e-38, 1e-33, 1e-20, 1e20, 1e35])
+def test_int8_rows_of_tiny_and_huge_weights(C, w):
+    require_gpu()
+    from telefuser_amd.norm import block_norm
+
+    x = _x((5, C), 1, BF16)
+    x[3] = 0.0  # beside the others in its wave
+    weight = torch.full((C,), w, device="cuda")
+    rows = block_norm(x, weight, norm="rms", out_dtype=torch.int8)
+    _, _, z, err = P.block(x, weight=weight, norm_kind="rms")
+    keep = torch.tensor([0, 1, 2, 4], device="cuda")
+    # a scale near the smallest float32 has few bits: the codes, not their products with it
+    top = z.abs().amax(-1, keepdim=True)
+    d = (rows.codes[keep, :C].double() - 127 * z[keep] / top[keep]).abs()
+    assert (d <= 0.5 + 127 * (err / top)[keep] * 2 + 127 * 8 * P.U32).all()
+    assert (rows.codes[3] == 0).all() and rows.scale[3] == 0
+    assert torch.isfinite(rows.scale).all()
+
+
 def test_constant_rows_and_large_means():
     require_gpu()
     from telefuser_amd.norm import block_norm
