@@ -46,10 +46,10 @@ struct LinearParams {
 };
 
 constexpr int kLinK = 128;  // bytes of K per stage
-// Tiles are walked down kLinGroup rows of them, then across: an XCD's 32 CUs share few rows of x and the weight passes by
-// all XCDs at once (75600 x 13824 x 5120, group 1 / 2 / 3 / 4 / 8: 4.84 / 4.14 / 4.10 / 4.6 / 4.8 ms; narrower
-// products prefer 2 to 4 too).
-constexpr int kLinGroup = 3;
+// Tiles are walked down this many rows of them, then across: an XCD's 32 CUs share few rows of x and the weight passes by
+// all XCDs at once (75600 x 13824 x 5120 in large tiles, group 1 / 2 / 3 / 4 / 8: 4.84 / 4.14 / 4.10 / 4.6 / 4.8 ms; 1560 x
+// 1536 x 8960 in small ones, 1 / 3 / 5 / 13: 34.5 / 31.0 / 29.8 / 30.8 us).
+constexpr int lin_group(int tile) { return tile == 256 ? 3 : 5; }
 
 template <int ACT>
 __device__ __forceinline__ float activate(float y) {
@@ -106,10 +106,11 @@ __device__ __forceinline__ void store_out8(char* o, int dtype, int64_t left, con
 template <int TM, int TN>
 __device__ __forceinline__ void place_tile(const LinearParams& p, int slot, int tiles, int64_t& m0, int64_t& n0) {
   const uint32_t id = (uint32_t)xcd_remap(slot, tiles);
-  const uint32_t per = kLinGroup * p.tiles_n, g = id / per, in = id - g * per;
-  const uint32_t gm = min((uint32_t)kLinGroup, (uint32_t)p.tiles_m - g * kLinGroup);
+  constexpr uint32_t kGroup = lin_group(TM);
+  const uint32_t per = kGroup * p.tiles_n, g = id / per, in = id - g * per;
+  const uint32_t gm = min(kGroup, (uint32_t)p.tiles_m - g * kGroup);
   const uint32_t tn = in / gm;
-  m0 = (int64_t)(g * kLinGroup + in - tn * gm) * TM;
+  m0 = (int64_t)(g * kGroup + in - tn * gm) * TM;
   n0 = (int64_t)tn * TN;
 }
 

@@ -42,9 +42,7 @@ class Int8Weight:
             raise ValueError("codes, scale and bias must be on one device")
         kpad = -(-k // 128) * 128
         if kpad != k:
-            padded = torch.zeros((n, kpad), dtype=torch.int8, device=dev)
-            padded[:, :k] = codes
-            codes = padded
+            codes = torch.nn.functional.pad(codes, (0, kpad - k))
         self.codes = codes if codes.is_contiguous() and codes.data_ptr() % 16 == 0 else codes.clone(
             memory_format=torch.contiguous_format)
         self.scale = scale.detach().reshape(n).to(torch.float32).contiguous()
