@@ -526,7 +526,8 @@ int qattn_norm_rope_stats(qattn_seq xq, qattn_seq xk, int dtype, int64_t B, int6
  * rint(127 z / max|z|) in rows of z_pitch bytes (a multiple of 16; C .. z_pitch is written 0) and z_scale[b * L + l] =
  * max|z| / 127.  A row of zeros has scale 0, one with an infinity or a NaN scale NaN and codes 0.  With norm NONE and
  * neither y nor parameters it is the row quantizer of activations (per token) and of weights (per channel).
- * At most 2^25 waves a launch: 2^25 rows, fewer of wide ones.  Outputs must not overlap inputs.
+ * At most 2^25 waves a launch: 2^25 rows, fewer of wide ones.  Outputs are 16-byte aligned and do
+ * not overlap inputs.
  * Parameters are fp32, bf16 or fp16 with the strides of their broadcast shape (0 along a dimension of one) and
  * contiguous channels; null: left out.
  */

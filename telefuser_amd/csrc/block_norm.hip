@@ -254,8 +254,8 @@ struct StagedParams {
   }
 };
 
-// One row; `first` is the thread's first channel, `step` the distance between its groups.  A group i of which no thread's
-// lies past the row's end (a condition on scalars) takes no masks.
+// A thread's part of a row as loaded; `first` is its first channel, `step` the distance between its groups.  A group i of
+// which no thread's lies past the row's end (a condition on scalars) takes no masks.
 template <int XD, int YM, int NV>
 struct RowValues {
   static constexpr int YD = YM == Y_BF16 ? QATTN_BF16 : YM == Y_FP16 ? QATTN_FP16 : XD;
@@ -272,7 +272,7 @@ struct RowValues {
   }
 };
 
-// r: the row's values, loaded; next() is called once they are used and may load others into r.
+// One row.  r: its values, loaded; next() is called once they are used and may load others into r.
 template <int XD, int YM, int NV, typename REDUCE, typename PARAMS, typename NEXT>
 __device__ __forceinline__ void norm_row(const BlockNormParams& p, int64_t b, int64_t l, int first, int step, REDUCE red,
                                          const PARAMS& params, const RowValues<XD, YM, NV>& r, NEXT next) {
@@ -574,7 +574,8 @@ static bool row_shape(int C, bool plain, int& waves, int& groups) {
 }
 
 // Staging pays from about this many rows of a batch entry (microseconds, read per row / staged: norm of 9000 x 5120 38.7 /
-// 43.7, of 20000 x 5120 96 / 85, of 75600 x 5120 365 / 306; gated residual + norm of 75600 x 640 111 / 85, of 48306 x 7040 685 / 516).
+// 43.7, of 20000 x 5120 96 / 85, of 75600 x 5120 365 / 306; gated residual + norm of 75600 x 640 111 / 85, of 48306 x 7040
+// 685 / 516).
 constexpr int64_t kStagedRows = 16384;
 constexpr int kStagedWidest = 8192;
 constexpr size_t kLds = 163840, kSlotBytes = 8 * 2 * 5 * kMaxRowWaves * 4;
@@ -672,7 +673,8 @@ extern "C" int qattn_block_norm(const qattn_block_norm_args* a, qattn_stream_t s
   p.h = a->h, p.z = a->z, p.z_scale = a->z_scale, p.z_pitch = a->z_pitch;
   p.x_dtype = a->x_dtype, p.y_dtype = a->y_dtype, p.z_dtype = a->z_dtype;
   Param* to[] = {&p.gate, &p.weight, &p.bias, &p.scale, &p.shift, &p.post_weight, &p.post_bias};
-  for (int i = 0; i < 7; i++) *to[i] = Param{params[i]->data, params[i]->dtype, a->B > 1 ? params[i]->sb : 0, a->L > 1 ? params[i]->sl : 0};
+  for (int i = 0; i < 7; i++)
+    *to[i] = Param{params[i]->data, params[i]->dtype, a->B > 1 ? params[i]->sb : 0, a->L > 1 ? params[i]->sl : 0};
   p.L = a->L, p.rows = a->B * a->L, p.C = (int)a->C;
   p.norm = a->norm, p.post_norm = a->y ? a->post_norm : QATTN_NORM_NONE;
   p.eps = a->eps, p.post_eps = a->post_eps, p.residual_scale = a->residual_scale;

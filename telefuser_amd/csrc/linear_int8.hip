@@ -19,8 +19,10 @@
 //     64 contiguous bytes for the four lanes of a token and its whole line in two stores (stores of 16 bytes at a stride
 //     of 32: 245 us there).
 //   * Scales and bias of a tile come into LDS by DMA with its first stage, four tiles deep.
-// Tiles: 256 x 256, two stages (stages double-buffered fill 128 KiB); 128 x 128, four stages, where the large tile leaves
-// CUs without work.  Rows past M or N lie behind the end of the buffer resource and read as zeros; so does every stage
+// Tiles: 256 x 256, two stages (they fill 128 KiB); 128 x 128 and 64 x 64, four stages, where larger ones leave CUs without
+// work.  A stage of the 128 x 128 tile takes about 950 cycles for 512 of MFMA (without the MFMAs 32.4 of 34.5 us at 1560 x
+// 1536 x 8960, without the LDS reads 29.4, without the DMA 25.8): the 32 KiB that a CU fetches for it bound it, and the tiny
+// tile fetches twice as much for its products.  Rows past M or N lie behind the end of the buffer resource and read as zeros; so does every stage
 // past the last.
 // 75600 x 13824 x 5120 4.10 ms (2.61 PFLOP/s), 32760 x 1536 x 8960 377 us (2.40), 32760 x 4608 x 1536 208 us (2.23).
 #include "attn_device.h"
@@ -117,9 +119,9 @@ __device__ __forceinline__ void place_tile(const LinearParams& p, int slot, int 
 // ACT = kSplit: a workgroup multiplies split_stages stages of a tile and leaves the int32 sums in p.part, each register of
 // the wave as one 1 KiB line.
 constexpr int kSplit = -1;
-template <int TM, int TN, int NB, int ACT>
+template <int TM, int TN, int WM, int NB, int ACT>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) void linear_int8_kernel(LinearParams p) {
-  constexpr int WM = 2, WN = 4, kWaves = WM * WN;
+  constexpr int kWaves = 8, WN = kWaves / WM;
   constexpr int NI = TN / WN / 16, MJ = TM / WM / 16;  // 16 x 16 results of a wave
   constexpr int kStage = (TM + TN) * kLinK;
   constexpr int IX = TM / 8 / kWaves, IW = TN / 8 / kWaves;  // DMA instructions of a wave and stage, 8 rows each
@@ -286,11 +288,12 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 }
 
-// The sums of the splits of a 128 x 128 tile, and what the tile kernel does with them at its end.  A wave takes what one
-// wave of the tile kernel left of 16 tokens.
-template <int ACT>
+// The sums of the splits of a tile, and what the tile kernel does with them at its end.  A wave takes what one wave of the
+// tile kernel left of 16 tokens.
+template <int TM, int TN, int WM, int ACT>
 __global__ __launch_bounds__(256) void linear_join_kernel(LinearParams p, int splits) {
-  constexpr int TM = 128, TN = 128, WM = 2, WN = 4, NI = TN / WN / 16, MJ = TM / WM / 16;
+  constexpr int WN = 8 / WM, NI = TN / WN / 16, MJ = TM / WM / 16;
+  static_assert(NI == 2);
   const int lane = threadIdx.x & 63, id = blockIdx.x * 4 + (threadIdx.x >> 6);
   const int tiles = p.tiles_m * p.tiles_n;
   const int j = id % MJ, wave = id / MJ % 8, slot = id / (MJ * 8);
@@ -492,13 +495,13 @@ static int launch_few(const FewParams& f, hipStream_t stream) {
   return f.lin.N >= 32 * 256 ? launch_few<2, X>(f, stream) : launch_few<1, X>(f, stream);
 }
 
-template <int TM, int TN, int NB>
+template <int TM, int TN, int WM, int NB>
 static int launch_linear(LinearParams& p, int workgroups, hipStream_t stream) {
   p.tiles_m = (int)((p.M + TM - 1) / TM), p.tiles_n = (int)((p.N + TN - 1) / TN);
   const dim3 grid((unsigned)std::min(p.tiles_m * p.tiles_n, workgroups)), block(512);
-  if (p.act == QATTN_ACT_GELU_TANH) linear_int8_kernel<TM, TN, NB, QATTN_ACT_GELU_TANH><<<grid, block, 0, stream>>>(p);
-  else if (p.act == QATTN_ACT_SILU) linear_int8_kernel<TM, TN, NB, QATTN_ACT_SILU><<<grid, block, 0, stream>>>(p);
-  else linear_int8_kernel<TM, TN, NB, QATTN_ACT_NONE><<<grid, block, 0, stream>>>(p);
+  if (p.act == QATTN_ACT_GELU_TANH) linear_int8_kernel<TM, TN, WM, NB, QATTN_ACT_GELU_TANH><<<grid, block, 0, stream>>>(p);
+  else if (p.act == QATTN_ACT_SILU) linear_int8_kernel<TM, TN, WM, NB, QATTN_ACT_SILU><<<grid, block, 0, stream>>>(p);
+  else linear_int8_kernel<TM, TN, WM, NB, QATTN_ACT_NONE><<<grid, block, 0, stream>>>(p);
   return check_launch("linear_int8");
 }
 
@@ -517,7 +520,7 @@ static int linear_params(LinearParams& p, const int8_t* w, int64_t w_pitch, cons
                 "linear_int8: K = %lld must be a multiple of 128 up to 131072 (int32 sums)", (long long)K);
   QATTN_REQUIRE(act >= QATTN_ACT_NONE && act <= QATTN_ACT_SILU, QATTN_ERR_ARG, "linear_int8: act code %d", act);
   if (M == 0) return QATTN_OK;
-  QATTN_REQUIRE(tiles_of(M, N, 128) < ((int64_t)1 << 23), QATTN_ERR_SHAPE, "linear_int8: more than 2^23 tiles");
+  QATTN_REQUIRE(tiles_of(M, N, 64) < ((int64_t)1 << 23), QATTN_ERR_SHAPE, "linear_int8: more than 2^23 tiles of 64 x 64");
   QATTN_REQUIRE(w && w_scale && out, QATTN_ERR_ARG, "linear_int8: a null operand");
   QATTN_REQUIRE(w_pitch >= K && w_pitch % 16 == 0 && w_pitch <= (1 << 22), QATTN_ERR_STRIDE,
                 "linear_int8: w_pitch %lld must be a multiple of 16 from K to 2^22", (long long)w_pitch);
@@ -530,49 +533,67 @@ static int linear_params(LinearParams& p, const int8_t* w, int64_t w_pitch, cons
   return QATTN_OK;
 }
 
-// Which kernel, by estimated microseconds (tile kernels: per stage and round of the chip, and 2 to start and end).
-enum LinearKernel { LINEAR_FEW, LINEAR_LARGE, LINEAR_SMALL };
+// Which kernel, by estimated microseconds: of a stage and of a tile's beginning and end, times the rounds of the chip; a
+// split along K writes its int32 sums and the join reads them (5 TB/s, and 3 us for its launch).  Measured, large / small /
+// tiny tile: 3000 x 3000 x 3000 38 / 42 / -, 32760 x 4608 x 1536 208 / 338 / -, 1560 x 1536 x 8960 85 / 30 / 46, 512 x 5120 x
+// 4096 43 / 17 / 26, 600 x 1536 x 1536 19 / 8.3 / 6.1, 777 x 999 x 1027 - / 9.7 / 5.7, 1000 x 640 x 4096 - / 15.6 / 9.6.
+enum LinearKernel { LINEAR_FEW, LINEAR_LARGE, LINEAR_SMALL, LINEAR_TINY };
 struct LinearPlan {
   LinearKernel kernel;
   int splits, split_stages;
 };
+static int64_t plan_tiles(const LinearPlan& plan, int64_t M, int64_t N) {
+  return tiles_of(M, N, plan.kernel == LINEAR_SMALL ? 128 : 64);
+}
 static LinearPlan plan_linear(int64_t M, int64_t N, int64_t K) {
   if (M <= kFewRows) return {LINEAR_FEW, 1, 0};
-  // a stage of the large tile takes 1.2 us (1.6 at the power limit), of the small one 0.46 (1560 x 1536 x 8960: 85 / 32
-  // us; 512 x 5120 x 4096: 43 / 17)
-  const int64_t large = tiles_of(M, N, 256), small = tiles_of(M, N, 128), stages = K / kLinK;
-  if ((large + kLinCus - 1) / kLinCus * 120 <= (small + kLinCus - 1) / kLinCus * 46) return {LINEAR_LARGE, 1, 0};
-  auto rounds = [&](int64_t workgroups, int64_t stages) {
-    return (double)((workgroups + kLinCus - 1) / kLinCus) * (0.46 * stages + 2);
+  const int64_t stages = K / kLinK;
+  auto cost = [](int64_t workgroups, int64_t stages, double stage, double ends) {
+    return (double)((workgroups + kLinCus - 1) / kLinCus) * (stage * stages + ends);
   };
-  LinearPlan best{LINEAR_SMALL, 1, (int)stages};
-  double least = 0.9 * rounds(small, stages);
-  for (int64_t s = 2; s <= 16 && s * small <= 2 * kLinCus && s * 4 <= stages; s++) {
-    // splits write their int32 sums, the join reads them: 5 TB/s, and 3 us for its launch
-    const int64_t per = (stages + s - 1) / s, splits = (stages + per - 1) / per;
-    const double t = rounds(splits * small, per) + 3 + 8.0 * splits * M * N / 5e6;
-    if (t < least) least = t, best = {LINEAR_SMALL, (int)splits, (int)per};
+  LinearPlan best{LINEAR_LARGE, 1, (int)stages};
+  double least = cost(tiles_of(M, N, 256), stages, 1.3, 5.0);
+  for (const LinearKernel kernel : {LINEAR_SMALL, LINEAR_TINY}) {
+    const double stage = kernel == LINEAR_SMALL ? 0.42 : 0.18, ends = kernel == LINEAR_SMALL ? 3.5 : 3.1;
+    const int64_t tiles = tiles_of(M, N, kernel == LINEAR_SMALL ? 128 : 64);
+    const double whole = cost(tiles, stages, stage, ends);
+    if (whole < least) least = whole, best = {kernel, 1, (int)stages};
+    for (int64_t s = 2; s <= 16 && s * tiles <= 2 * kLinCus && s * 4 <= stages; s++) {
+      const int64_t per = (stages + s - 1) / s, splits = (stages + per - 1) / per;
+      const double t = (cost(splits * tiles, per, stage, ends) + 3 + 8.0 * splits * M * N / 5e6) / 0.9;
+      if (t < least) least = t, best = {kernel, (int)splits, (int)per};
+    }
   }
   return best;
 }
 static size_t split_bytes(const LinearPlan& plan, int64_t M, int64_t N) {
-  return plan.splits > 1 ? (size_t)plan.splits * tiles_of(M, N, 128) * 128 * 128 * 4 : 0;
+  const size_t tile = plan.kernel == LINEAR_SMALL ? 128 : 64;
+  return plan.splits > 1 ? plan.splits * plan_tiles(plan, M, N) * tile * tile * 4 : 0;
+}
+
+template <int TM, int TN, int WM, int NB>
+static int launch_split(LinearParams& p, const LinearPlan& plan, void* workspace, hipStream_t stream) {
+  p.part = static_cast<v4i*>(workspace), p.split_stages = plan.split_stages;
+  p.tiles_m = (int)((p.M + TM - 1) / TM), p.tiles_n = (int)((p.N + TN - 1) / TN);
+  const int tiles = p.tiles_m * p.tiles_n;
+  linear_int8_kernel<TM, TN, WM, NB, kSplit><<<dim3((unsigned)(tiles * plan.splits)), dim3(512), 0, stream>>>(p);
+  if (int rc = check_launch("linear_int8")) return rc;
+  // one wave for each of a tile's eight and each of its groups of 16 tokens
+  const dim3 grid((unsigned)(tiles * 2 * (TM / WM / 16))), block(256);
+  if (p.act == QATTN_ACT_GELU_TANH) linear_join_kernel<TM, TN, WM, QATTN_ACT_GELU_TANH><<<grid, block, 0, stream>>>(p, plan.splits);
+  else if (p.act == QATTN_ACT_SILU) linear_join_kernel<TM, TN, WM, QATTN_ACT_SILU><<<grid, block, 0, stream>>>(p, plan.splits);
+  else linear_join_kernel<TM, TN, WM, QATTN_ACT_NONE><<<grid, block, 0, stream>>>(p, plan.splits);
+  return check_launch("linear_int8");
 }
 
 static int run_linear(LinearParams& p, const LinearPlan& plan, void* workspace, hipStream_t stream) {
   if (plan.kernel == LINEAR_FEW) return launch_few<-1>(FewParams{p, nullptr, 0, 0, 1, 0, false}, stream);
-  if (plan.kernel == LINEAR_LARGE) return launch_linear<256, 256, 2>(p, kLinCus, stream);
-  if (plan.splits == 1) return launch_linear<128, 128, 4>(p, INT32_MAX, stream);
-  p.part = static_cast<v4i*>(workspace), p.split_stages = plan.split_stages;
-  p.tiles_m = (int)((p.M + 127) / 128), p.tiles_n = (int)((p.N + 127) / 128);
-  const int tiles = p.tiles_m * p.tiles_n;
-  linear_int8_kernel<128, 128, 4, kSplit><<<dim3((unsigned)(tiles * plan.splits)), dim3(512), 0, stream>>>(p);
-  if (int rc = check_launch("linear_int8")) return rc;
-  const dim3 grid((unsigned)(tiles * 8)), block(256);
-  if (p.act == QATTN_ACT_GELU_TANH) linear_join_kernel<QATTN_ACT_GELU_TANH><<<grid, block, 0, stream>>>(p, plan.splits);
-  else if (p.act == QATTN_ACT_SILU) linear_join_kernel<QATTN_ACT_SILU><<<grid, block, 0, stream>>>(p, plan.splits);
-  else linear_join_kernel<QATTN_ACT_NONE><<<grid, block, 0, stream>>>(p, plan.splits);
-  return check_launch("linear_int8");
+  if (plan.kernel == LINEAR_LARGE) return launch_linear<256, 256, 2, 2>(p, kLinCus, stream);
+  if (plan.splits > 1)
+    return plan.kernel == LINEAR_SMALL ? launch_split<128, 128, 2, 4>(p, plan, workspace, stream)
+                                       : launch_split<64, 64, 4, 4>(p, plan, workspace, stream);
+  return plan.kernel == LINEAR_SMALL ? launch_linear<128, 128, 2, 4>(p, INT32_MAX, stream)
+                                     : launch_linear<64, 64, 4, 4>(p, INT32_MAX, stream);
 }
 
 static int check_workspace(const void* workspace, size_t bytes, size_t need) {

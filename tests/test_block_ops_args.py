@@ -190,7 +190,7 @@ def test_linear_workspaces(lib):
     assert rows(1, 64, 16385) == 16528 and rows(99, 64, 200) == 99 * 260 + 4 and rows(75600, 64, 5120) == 75600 * 5124
     # split along K: few tiles and many stages, whole tiles of int32 sums
     assert split(75600, 13824, 5120) == split(1560, 1536, 8960) == split(200, 64, 256) == split(16, 64, 8960) == 0
-    for m, n, k in ((17, 100, 4096), (64, 1536, 8960), (100, 9216, 13824)):
-        tiles = -(-m // 128) * -(-n // 128)
-        assert split(m, n, k) % (tiles * 128 * 128 * 4) == 0 and 2 <= split(m, n, k) // (tiles * 128 * 128 * 4) <= 16
+    for m, n, k in ((17, 100, 4096), (64, 1536, 8960), (100, 9216, 13824), (300, 300, 13824)):
+        tile = -(-m // 64) * -(-n // 64) * 64 * 64 * 4  # (a larger tile holds whole ones of these)
+        assert split(m, n, k) >= 2 * tile and split(m, n, k) % (64 * 64 * 4) == 0
         assert rows(m, n, k) == (m * k + m * 4 + 15) // 16 * 16 + split(m, n, k)

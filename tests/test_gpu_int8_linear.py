@@ -29,10 +29,11 @@ def _check(x, w, act, out, what):
     P.check(out, ref, err, what)
 
 
-SIZES = [(1, 1, 1), (1, 128, 3), (1, 1536, 1536), (2, 129, 33), (3, 64, 5120), (5, 4096, 64), (8, 640, 200), (15, 1027, 129), (16, 256, 17),
-         (17, 128, 64), (31, 300, 100), (33, 127, 65), (64, 512, 96), (65, 256, 128), (100, 2048, 129), (127, 128, 999),
+SIZES = [(1, 1, 1), (1, 128, 3), (1, 1536, 1536), (2, 129, 33), (3, 64, 5120), (5, 4096, 64), (8, 640, 200), (15, 1027, 129),
+         (16, 256, 17), (17, 128, 64), (31, 300, 100), (33, 127, 65), (64, 512, 96), (65, 256, 128), (100, 2048, 129), (127, 128, 999),
          (128, 1536, 256), (129, 256, 513), (200, 8960, 96), (255, 384, 257), (256, 128, 256), (257, 1024, 640),
-         (300, 1027, 999), (600, 128, 1100), (1024, 512, 513), (1560, 640, 1536), (2049, 256, 1025)]
+         (300, 1027, 999), (600, 128, 1100), (1024, 512, 513), (1560, 640, 1536), (2049, 256, 1025),
+         (1300, 2000, 1537), (2500, 13824, 640), (3000, 300, 3001), (9000, 200, 4000)]
 
 
 @pytest.mark.parametrize("M,K,N", SIZES)
