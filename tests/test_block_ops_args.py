@@ -194,3 +194,26 @@ def test_linear_workspaces(lib):
         tile = -(-m // 64) * -(-n // 64) * 64 * 64 * 4  # (a larger tile holds whole ones of these)
         assert split(m, n, k) >= 2 * tile and split(m, n, k) % (64 * 64 * 4) == 0
         assert rows(m, n, k) == (m * k + m * 4 + 15) // 16 * 16 + split(m, n, k)
+
+
+@pytest.mark.parametrize("current,index,entered", [(0, 0, []), (0, 2, [2]), (1, 0, [0])])
+def test_launch_on_the_tensors_device(monkeypatch, current, index, entered):
+    """A launch takes the current stream of the tensors' GPU, with that GPU made current for it if it is not."""
+    seen, inside = [], []
+
+    class Device:
+        def __init__(self, i):
+            self.i = i
+
+        def __enter__(self):
+            inside.append(self.i)
+
+        def __exit__(self, *exc):
+            inside.append("left")
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 1000 + i, raising=False)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    _lib.launch(index, lambda *a: seen.append((a, list(inside))), "x", 5)
+    assert seen == [(("x", 5, 1000 + index), entered)]
+    assert inside == (entered + ["left"] if entered else [])
