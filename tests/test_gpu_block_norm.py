@@ -161,6 +161,23 @@ def test_per_token_int8(M, K, dtype):
     assert d.shape == x.shape and ((d.double() - x.double()).abs() <= scale[:, None] * 0.5001).all()
 
 
+@pytest.mark.parametrize("dtype,bits", [(FP16, 10), (BF16, 7)])
+def test_codes_of_every_pair_of_half_values(dtype, bits):
+    """A row for every mantissa of the maximum, holding every mantissa at the ten exponents below it (values further below
+    have code 0): the codes are those of the real numbers."""
+    require_gpu()
+    from telefuser_amd.norm import per_token_int8
+
+    m = 1 + torch.arange(2 ** bits, device="cuda", dtype=torch.float64) / 2 ** bits
+    x = torch.cat([m * 2.0 ** -e for e in range(10)]).expand(len(m), -1)
+    x = torch.where(x <= m[:, None], x, 0.0)
+    x = torch.cat([m[:, None], x, -x], 1).to(dtype)
+    rows = per_token_int8(x)
+    codes, scale = P.codes_of(x)
+    assert torch.equal(rows.scale, scale.float())
+    assert torch.equal(rows.codes[:, :x.shape[1]].double(), codes)
+
+
 @pytest.mark.parametrize("K", [8, 100, 1536, 9000])
 def test_int8_rows_of_extreme_values(K):
     require_gpu()
