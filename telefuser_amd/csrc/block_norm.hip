@@ -321,11 +321,9 @@ __device__ __forceinline__ void norm_row(const BlockNormParams& p, int64_t b, in
         float mul[8], add[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) v[i][e] *= rstd;
-        if (params.post(first + i * step, whole(i), mul, add)) {
-          const int left = whole(i) ? 8 : C - first - i * step;  // past the row's end stay zeros: the next norm sums them
+        if (params.post(first + i * step, whole(i), mul, add))
 #pragma unroll
-          for (int e = 0; e < 8; e++) v[i][e] = e < left ? fmaf(v[i][e], mul[e], add[e]) : 0.0f;
-        }
+          for (int e = 0; e < 8; e++) v[i][e] = fmaf(v[i][e], mul[e], add[e]);
       }
     }
 #pragma unroll
@@ -336,6 +334,12 @@ __device__ __forceinline__ void norm_row(const BlockNormParams& p, int64_t b, in
         for (int e = 0; e < 8; e++) v[i][e] *= t[e];
 #pragma unroll
       for (int e = 0; e < 8; e++) v[i][e] = fmaf(p.residual_scale, r.x[i].get(e), v[i][e]);
+      if (!whole(i)) {  // past the row's end stay zeros, whatever the parameters made of them: the next norm sums them
+        const int left = C - first - i * step;
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (e >= left) v[i][e] = 0.0f;
+      }
     }
   } else {
 #pragma unroll

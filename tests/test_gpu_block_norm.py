@@ -292,6 +292,21 @@ def test_many_rows_of_shared_parameters(B, L, C, dtype):
         assert ((full[:, i:i + 8000].float() - part.float()).abs() <= 0.02 * (part.float().abs() + 1)).all()
 
 
+@pytest.mark.parametrize("C", [260, 1027, 1536])
+@pytest.mark.parametrize("L", [40, 16384])
+def test_infinite_gate_of_the_last_channel(L, C):
+    """The lanes past a row's end keep zeros: an infinite value leaves 0 in the other channels of an RMS norm, NaN in its
+    own."""
+    require_gpu()
+    from telefuser_amd.norm import gated_residual_norm
+
+    x, y, gate = _x((1, L, C), 1, BF16), _x((1, L, C), 2, BF16).abs() + 1, _p((C,), 3)
+    gate[-1] = float("inf")
+    h, z = gated_residual_norm(x, y, gate, norm="rms")
+    assert (h[..., -1] == float("inf")).all() and z[..., -1].isnan().all()
+    assert h[..., :-1].isfinite().all() and (z[..., :-1] == 0).all()
+
+
 def test_offsets_past_32_bits():
     require_gpu()
     from telefuser_amd.norm import gated_residual_norm
