@@ -116,6 +116,7 @@ def _linear_rows(lib, x: Int8Rows, weight: Int8Weight, act_code: int, out_dtype)
     if codes.dtype != torch.int8 or x_scale.dtype != torch.float32 or codes.shape[:-1] != x_scale.shape or \
             not codes.is_contiguous() or not x_scale.is_contiguous() or x_scale.get_device() != dev:
         raise ValueError("Int8Rows must hold contiguous int8 codes and a contiguous float32 scale for each row")
+    _no_grad(x_scale)
     if not codes.is_cuda or weight.codes.get_device() != dev:
         raise ValueError(f"x is on {codes.device}, the weight on {weight.codes.device}: both must be on one GPU")
     out = codes.new_empty((*codes.shape[:-1], n), dtype=out_dtype)

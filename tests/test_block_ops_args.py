@@ -70,6 +70,7 @@ def test_weight_layout():
     (Int8Rows(torch.zeros(2, 128, dtype=torch.int8), torch.ones(2).double(), 64), {}, "float32 scale"),
     (Int8Rows(torch.zeros(2, 256, dtype=torch.int8)[:, :128], torch.ones(2), 64), {}, "contiguous"),
     (Int8Rows(torch.zeros(2, 128), torch.ones(2), 64), {}, "int8 codes"),
+    (Int8Rows(torch.zeros(2, 128, dtype=torch.int8), torch.ones(2, requires_grad=True), 64), {}, "no backward"),
 ])
 def test_linear_refusals(rows, kw, words):
     with pytest.raises(ValueError, match=words):
