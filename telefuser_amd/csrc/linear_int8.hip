@@ -19,11 +19,12 @@
 //     64 contiguous bytes for the four lanes of a token and its whole line in two stores (stores of 16 bytes at a stride
 //     of 32: 245 us there).
 //   * Scales and bias of a tile come into LDS by DMA with its first stage, four tiles deep.
-// Tiles: 256 x 256, two stages (they fill 128 KiB); 128 x 128 and 64 x 64, four stages, where larger ones leave CUs without
-// work.  A stage of the 128 x 128 tile takes about 950 cycles for 512 of MFMA (without the MFMAs 32.4 of 34.5 us at 1560 x
-// 1536 x 8960, without the LDS reads 29.4, without the DMA 25.8): the 32 KiB that a CU fetches for it bound it, and the tiny
-// tile fetches twice as much for its products.  Rows past M or N lie behind the end of the buffer resource and read as zeros; so does every stage
-// past the last.
+// Tiles: 256 x 256, two stages (they fill 128 KiB); 128 x 128, three (512 x 5120 x 4096 17.6 us, with four 18.0), and 64 x
+// 64, four (39606 x 64 x 3328 26.5 us, with three 28.1), where larger ones leave CUs without work.  A stage of the 128 x 128
+// tile takes about 950 cycles for 512 of MFMA; reads, DMA and MFMAs overlap in part (without the MFMAs 32.4 of 34.5 us at
+// 1560 x 1536 x 8960, without the LDS reads 29.4, without the DMA 25.8).  96 x 128 tiles, on 204 CUs there instead of 156,
+// fetch a seventh more in all and take the same time.  The tiny tile fetches twice as much for its products.  Rows past M or
+// N lie behind the end of the buffer resource and read as zeros; so does every stage past the last.
 // 75600 x 13824 x 5120 4.10 ms (2.61 PFLOP/s), 32760 x 1536 x 8960 377 us (2.40), 32760 x 4608 x 1536 208 us (2.23).
 #include "attn_device.h"
 
@@ -598,9 +599,9 @@ static int run_linear(LinearParams& p, const LinearPlan& plan, void* workspace, 
   if (plan.kernel == LINEAR_FEW) return launch_few<-1>(FewParams{p, nullptr, 0, 0, 1, 0, false}, stream);
   if (plan.kernel == LINEAR_LARGE) return launch_linear<256, 256, 2, 2>(p, kLinCus, stream);
   if (plan.splits > 1)
-    return plan.kernel == LINEAR_SMALL ? launch_split<128, 128, 2, 4>(p, plan, workspace, stream)
+    return plan.kernel == LINEAR_SMALL ? launch_split<128, 128, 2, 3>(p, plan, workspace, stream)
                                        : launch_split<64, 64, 4, 4>(p, plan, workspace, stream);
-  return plan.kernel == LINEAR_SMALL ? launch_linear<128, 128, 2, 4>(p, INT32_MAX, stream)
+  return plan.kernel == LINEAR_SMALL ? launch_linear<128, 128, 2, 3>(p, INT32_MAX, stream)
                                      : launch_linear<64, 64, 4, 4>(p, INT32_MAX, stream);
 }
 
