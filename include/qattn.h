@@ -552,6 +552,11 @@ typedef struct qattn_block_norm_args {
   float eps, post_eps, residual_scale;
 } qattn_block_norm_args;
 int qattn_block_norm(const qattn_block_norm_args* args, qattn_stream_t stream);
+/*
+ * The same, and y may be fp32 beside an x of either half type: the output of qattn_linear_int8 then reaches the residual as
+ * it was computed, without a rounding to x's type between the two.
+ */
+int qattn_block_norm_ex(const qattn_block_norm_args* args, qattn_stream_t stream);
 
 /*
  * INT8 linear: out[m, n] = act(x_scale[m] * w_scale[n] * sum_k x[m, k] w[n, k] + bias[n]), the sum exact in int32.

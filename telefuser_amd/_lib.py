@@ -55,6 +55,7 @@ EXPORTED = (
     "qattn_v_tile_half_varlen",
     "qattn_fwd_varlen",
     "qattn_block_norm",
+    "qattn_block_norm_ex",
     "qattn_linear_int8_workspace_size",
     "qattn_linear_int8",
     "qattn_linear_int8_rows_workspace_size",
@@ -193,7 +194,9 @@ def load() -> ctypes.CDLL:
     L.qattn_v_tile_half_varlen.argtypes = [S, i32, i64, i64, i64, i64, i64, vp, vp, vp, i64, vp]
     L.qattn_fwd_varlen.argtypes = [S, vp, S, vp, vp, i64, S, i32, i64, i64, i64, i64, i64, i64, i64, i64, f32, i32, vp,
                                    vp, vp, vp, vp, vp]
-    L.qattn_block_norm.argtypes = [vp, vp]  # qattn_block_norm_args, as bytes or by reference
+    for name in ("qattn_block_norm", "qattn_block_norm_ex"):
+        getattr(L, name).argtypes = [vp, vp]  # qattn_block_norm_args, as bytes or by reference
+        getattr(L, name).restype = i32
     L.qattn_linear_int8_workspace_size.argtypes = [i64, i64, i64]
     L.qattn_linear_int8_workspace_size.restype = sz
     L.qattn_linear_int8.argtypes = [vp, i64, vp, vp, i64, vp, vp, vp, i32, i64, i64, i64, i64, i32, vp, sz, vp]
@@ -201,7 +204,7 @@ def load() -> ctypes.CDLL:
     L.qattn_linear_int8_rows_workspace_size.restype = sz
     L.qattn_linear_int8_rows.argtypes = [vp, i32, i64, i64, i64, i64, i64, vp, i64, vp, vp, vp, i32, i64, i64, i32, vp,
                                          sz, vp]
-    for name in ("qattn_block_norm", "qattn_linear_int8", "qattn_linear_int8_rows"):
+    for name in ("qattn_linear_int8", "qattn_linear_int8_rows"):
         getattr(L, name).restype = i32
     for name in ("qattn_norm_rope_stats", "qattn_sage_quant_half", "qattn_lse_finish", "qattn_v_tile_half_ex", "qattn_v_tile_half_varlen_ex", "qattn_varlen_offsets", "qattn_quant_qk_varlen_int8", "qattn_v_tile_half_varlen",
                  "qattn_fwd_varlen"):

@@ -64,7 +64,7 @@ __device__ __forceinline__ float load_param(const Param& q, int64_t b, int64_t l
 // A thread holds NV groups of 8 consecutive channels of a row: every value is loaded once, the reductions run over
 // registers, and the outputs are written from them.  A group is one 16-byte access (two for fp32) at whatever alignment
 // its row has; only a group that the row's end cuts goes element by element.
-enum YMode { Y_NONE, Y_SAME, Y_BF16, Y_FP16 };
+enum YMode { Y_NONE, Y_SAME, Y_BF16, Y_FP16, Y_F32 };
 
 typedef v4u v4u_any __attribute__((aligned(2)));  // rows of halves start anywhere
 typedef v4u v4u_word __attribute__((aligned(4)));
@@ -258,7 +258,7 @@ struct StagedParams {
 // which no thread's lies past the row's end (a condition on scalars) takes no masks.
 template <int XD, int YM, int NV>
 struct RowValues {
-  static constexpr int YD = YM == Y_BF16 ? QATTN_BF16 : YM == Y_FP16 ? QATTN_FP16 : XD;
+  static constexpr int YD = YM == Y_BF16 ? QATTN_BF16 : YM == Y_FP16 ? QATTN_FP16 : YM == Y_F32 ? QATTN_F32 : XD;
   RawGroup<XD> x[NV];
   RawGroup<YD> y[YM == Y_NONE ? 1 : NV];
   __device__ __forceinline__ void load(const BlockNormParams& p, int64_t b, int64_t l, int first, int step) {
@@ -584,7 +584,7 @@ constexpr int64_t kStagedRows = 16384;
 constexpr int kStagedWidest = 8192;
 constexpr size_t kLds = 163840, kSlotBytes = 8 * 2 * 5 * kMaxRowWaves * 4;
 // Groups a thread holds in the staged kernel, before a row takes two or four waves.
-constexpr int staged_groups(int dtype) { return dtype == QATTN_F32 ? 3 : 5; }
+constexpr int staged_groups(int dtype, int ymode) { return dtype == QATTN_F32 || ymode == Y_F32 ? 3 : 5; }
 constexpr int64_t kCus = 256;
 // Offsets of the folded parameters in LDS, and its bytes; 0 where rows do not share them or LDS does not hold
 // them.
@@ -606,7 +606,7 @@ static size_t stage(BlockNormParams& p, const Param* const* params) {
 template <int XD, int YM>
 static void launch_rows(const BlockNormParams& p, int waves, int groups, size_t lds, hipStream_t stream) {
   if (lds) {
-    const int vecs = (p.C + 511) / 512, nvmax = staged_groups(XD);
+    const int vecs = (p.C + 511) / 512, nvmax = staged_groups(XD, YM);
     const int w = vecs <= nvmax ? 1 : vecs <= 2 * nvmax ? 2 : 4, nv = (vecs + w - 1) / w;
     // rows of a batch entry in turns, as many workgroups as the CUs hold at once: two to a CU by their registers
     const int64_t batches = p.rows / p.L, per = 8 / w;
@@ -636,13 +636,15 @@ static void launch_rows(const BlockNormParams& p, int waves, int groups, size_t 
   else row_norm_kernel<XD, YM, 5><<<grid, block, 0, stream>>>(p);
 }
 
-extern "C" int qattn_block_norm(const qattn_block_norm_args* a, qattn_stream_t stream) {
+// any_y: y may also be fp32 beside a half x
+static int run_block_norm(const qattn_block_norm_args* a, bool any_y, qattn_stream_t stream) {
   QATTN_REQUIRE(a && a->size == sizeof(qattn_block_norm_args), QATTN_ERR_ARG,
                 "block_norm: args missing or of another version of the header");
   QATTN_REQUIRE(a->x_dtype >= QATTN_BF16 && a->x_dtype <= QATTN_F32, QATTN_ERR_DTYPE, "block_norm: x has dtype code %d",
                 a->x_dtype);
-  QATTN_REQUIRE(!a->y || a->y_dtype == a->x_dtype || (a->x_dtype == QATTN_F32 && a->y_dtype >= QATTN_BF16 &&
-                                                      a->y_dtype <= QATTN_F32),
+  QATTN_REQUIRE(!a->y || a->y_dtype == a->x_dtype ||
+                    (a->x_dtype == QATTN_F32 && a->y_dtype >= QATTN_BF16 && a->y_dtype <= QATTN_F32) ||
+                    (any_y && a->y_dtype == QATTN_F32),
                 QATTN_ERR_DTYPE, "block_norm: y has dtype code %d beside x's %d", a->y_dtype, a->x_dtype);
   QATTN_REQUIRE(!a->z || (a->z_dtype >= QATTN_BF16 && a->z_dtype <= QATTN_I8), QATTN_ERR_DTYPE,
                 "block_norm: z has dtype code %d", a->z_dtype);
@@ -700,11 +702,20 @@ extern "C" int qattn_block_norm(const qattn_block_norm_args* a, qattn_stream_t s
     else if (p.y_dtype == QATTN_BF16) launch_rows<QATTN_F32, Y_BF16>(p, waves, groups, lds, st);
     else launch_rows<QATTN_F32, Y_FP16>(p, waves, groups, lds, st);
   } else if (p.x_dtype == QATTN_BF16) {
-    if (p.y) launch_rows<QATTN_BF16, Y_SAME>(p, waves, groups, lds, st);
-    else launch_rows<QATTN_BF16, Y_NONE>(p, waves, groups, lds, st);
+    if (!p.y) launch_rows<QATTN_BF16, Y_NONE>(p, waves, groups, lds, st);
+    else if (p.y_dtype == QATTN_F32) launch_rows<QATTN_BF16, Y_F32>(p, waves, groups, lds, st);
+    else launch_rows<QATTN_BF16, Y_SAME>(p, waves, groups, lds, st);
   } else {
-    if (p.y) launch_rows<QATTN_FP16, Y_SAME>(p, waves, groups, lds, st);
-    else launch_rows<QATTN_FP16, Y_NONE>(p, waves, groups, lds, st);
+    if (!p.y) launch_rows<QATTN_FP16, Y_NONE>(p, waves, groups, lds, st);
+    else if (p.y_dtype == QATTN_F32) launch_rows<QATTN_FP16, Y_F32>(p, waves, groups, lds, st);
+    else launch_rows<QATTN_FP16, Y_SAME>(p, waves, groups, lds, st);
   }
   return check_launch("block_norm");
+}
+
+extern "C" int qattn_block_norm(const qattn_block_norm_args* args, qattn_stream_t stream) {
+  return run_block_norm(args, false, stream);
+}
+extern "C" int qattn_block_norm_ex(const qattn_block_norm_args* args, qattn_stream_t stream) {
+  return run_block_norm(args, true, stream);
 }

@@ -118,8 +118,8 @@ def _run(x, y, gate, residual_scale, post, post_weight, post_bias, post_eps, wan
         y_dt = _check_input(y, "y")
         if y.shape != shape or y.get_device() != dev:
             raise ValueError(f"y must be {tuple(shape)} on {x.device}, got {tuple(y.shape)} on {y.device}")
-        if y_dt != x_dt and x_dt != _lib.QATTN_F32:
-            raise ValueError(f"y must have x's dtype {x.dtype} (or x be float32), got {y.dtype}")
+        if y_dt != x_dt and _lib.QATTN_F32 not in (x_dt, y_dt):
+            raise ValueError(f"y must have x's dtype {x.dtype} (or one of them be float32), got {y.dtype}")
         yr, y_sb, y_sl = _rows(y)
         keep.append(yr)
         y_ptr = yr.data_ptr()
@@ -150,7 +150,7 @@ def _run(x, y, gate, residual_scale, post, post_weight, post_bias, post_eps, wan
             *(_NO_PARAM if post_weight is None else _param(post_weight, x, "post_weight", keep)),
             *(_NO_PARAM if post_bias is None else _param(post_bias, x, "post_bias", keep)),
             x_dt, y_dt, z_dt, _NORM[norm], _NORM[post], eps, post_eps, residual_scale)
-        _lib.launch(dev, _lib.load().qattn_block_norm, args)
+        _lib.launch(dev, _lib.load().qattn_block_norm_ex, args)
     return h, z
 
 
@@ -174,8 +174,9 @@ def gated_residual(x: torch.Tensor, y: torch.Tensor, gate: Optional[torch.Tensor
                    post_eps: float = 1e-6) -> torch.Tensor:
     """The residual after a block: residual_scale * x + gate * y in x's dtype, computed in float32.
 
-    y has x's shape and dtype (any of the three beside a float32 x); gate broadcasts against x.  post_norm ("layer" or
-    "rms", with post_weight and post_bias) normalizes y's rows first."""
+    y has x's shape, and its dtype or float32 (any of the three beside a float32 x); gate broadcasts against x.  post_norm
+    ("layer" or "rms", with post_weight and post_bias) normalizes y's rows first.  A float32 y, as
+    ``int8_linear(..., out_dtype=torch.float32)`` gives it, is not rounded on its way into the sum."""
     return _run(x, y, gate, residual_scale, _post(post_norm, post_weight, post_bias), post_weight, post_bias, post_eps,
                 True, None, None, None, None, None, 0.0, None)[0]
 
