@@ -242,8 +242,9 @@ def _run_own(s):
         return block_norm(s["x"], **how)
     if kind == "enter":
         return int8_linear(block_norm(s["x"], **how, out_dtype=torch.int8), s["weight"], out_dtype=s["x"].dtype)
-    if kind == "leave":
-        return gated_residual_norm(s["x"], int8_linear(s["y"], s["weight"]), s["gate"], **how)
+    if kind == "leave":  # the product reaches the sum in float32, as in the plain form
+        y = int8_linear(s["y"], s["weight"], out_dtype=torch.float32)
+        return gated_residual_norm(s["x"], y, s["gate"], **how)
     post = {} if s["post"] is None else {"post_norm": "rms", "post_weight": s["post"]}
     return gated_residual_norm(s["x"], s["y"], s["gate"], **post, **how)
 
