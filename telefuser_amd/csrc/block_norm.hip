@@ -149,6 +149,7 @@ __device__ __forceinline__ void store8(void* p, int dtype, int64_t at, int c, in
 // Reductions over the lanes of a row: LANES of a wave, or whole waves (each call then has its own LDS slots, so one
 // barrier separates write and read).
 constexpr int kMaxRowWaves = 8;
+constexpr int kRowSlots = 7;  // two LayerNorms of three sums, and the maximum
 template <int LANES>
 struct RowReduce {
   uint32_t (*slots)[kMaxRowWaves];
@@ -174,10 +175,23 @@ struct RowReduce {
       return t;
     }
   }
-  __device__ __forceinline__ float sum(float v) {
-    return __uint_as_float(reduce(__float_as_uint(v), [](uint32_t a, uint32_t b) {
-      return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
-    }));
+  static __device__ __forceinline__ uint32_t plus(uint32_t a, uint32_t b) {
+    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
+  }
+  __device__ __forceinline__ float sum(float v) { return __uint_as_float(reduce(__float_as_uint(v), plus)); }
+  // both at one barrier
+  __device__ __forceinline__ void sums(float& v, float& w) {
+    if (LANES < 64 || waves == 1) {
+      v = sum(v), w = sum(w);
+      return;
+    }
+    const uint32_t a = wave_reduce(__float_as_uint(v), 0u, plus), b = wave_reduce(__float_as_uint(w), 0u, plus);
+    uint32_t *s = slots[used], *t = slots[used + 1];
+    used += 2;
+    if ((threadIdx.x & 63) == 0) s[wave] = a, t[wave] = b;
+    __syncthreads();
+    v = __uint_as_float(s[0]), w = __uint_as_float(t[0]);
+    for (int i = 1; i < waves; i++) v += __uint_as_float(s[i]), w += __uint_as_float(t[i]);
   }
   __device__ __forceinline__ uint32_t top(uint32_t v) {
     return reduce(v, [](uint32_t a, uint32_t b) { return max(a, b); });
@@ -254,6 +268,12 @@ struct StagedParams {
   }
 };
 
+// 1 / sqrt(var + eps) from the mean square of values whose mean is `rest`; an infinite one stays
+__device__ __forceinline__ float inv_deviation(float square, float rest, float eps) {
+  const float var = square < __builtin_inff() ? fmaxf(fmaf(-rest, rest, square), 0.0f) : square;
+  return 1.0f / sqrtf(var + eps);
+}
+
 // A thread's part of a row as loaded; `first` is its first channel, `step` the distance between its groups.  A group i of
 // which no thread's lies past the row's end (a condition on scalars) takes no masks.
 template <int XD, int YM, int NV>
@@ -281,16 +301,18 @@ __device__ __forceinline__ void norm_row(const BlockNormParams& p, int64_t b, in
   const float inv_c = 1.0f / (float)C;
   auto whole = [&](int i) __attribute__((always_inline)) { return (i + 1) * step <= C; };
   float v[NV][8];
-  // v - mean (or v) in place and 1 / sqrt(var + eps); values past the row's end are zeros before and after
+  // v - mean (or v) in place and 1 / sqrt(var + eps); values past the row's end are zeros before, and anything after.  The
+  // mean of a float32 sum is off by a few roundings of its own size, which a row of small variance beside its mean would
+  // show (or a constant one, whose result is 0): what is left of it in the centred values, and of their variance, goes too.
   auto normalize = [&](int kind, float eps) __attribute__((always_inline)) {
-    float mean = 0.0f, s = 0.0f;
+    float s = 0.0f;
     if (kind == QATTN_NORM_LAYER) {
 #pragma unroll
       for (int i = 0; i < NV; i++)
 #pragma unroll
         for (int e = 0; e < 8; e++) s += v[i][e];
-      mean = red.sum(s) * inv_c;
-      s = 0.0f;
+      const float mean = red.sum(s) / (float)C;
+      float rest = 0.0f, var = 0.0f;
 #pragma unroll
       for (int i = 0; i < NV; i++) {
 #pragma unroll
@@ -301,7 +323,16 @@ __device__ __forceinline__ void norm_row(const BlockNormParams& p, int64_t b, in
           for (int e = 0; e < 8; e++)
             if (e >= left) v[i][e] = 0.0f;
         }
+#pragma unroll
+        for (int e = 0; e < 8; e++) rest += v[i][e], var = fmaf(v[i][e], v[i][e], var);
       }
+      red.sums(rest, var);
+      rest /= (float)C;
+#pragma unroll
+      for (int i = 0; i < NV; i++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) v[i][e] -= rest;
+      return inv_deviation(var * inv_c, rest, eps);
     }
 #pragma unroll
     for (int i = 0; i < NV; i++)
@@ -419,7 +450,7 @@ __global__ __launch_bounds__(256) void narrow_row_kernel(BlockNormParams p) {
 // A workgroup a row.
 template <int XD, int YM, int NV>
 __global__ __launch_bounds__(kMaxRowWaves * 64) void row_norm_kernel(BlockNormParams p) {
-  __shared__ uint32_t slots[5][kMaxRowWaves];
+  __shared__ uint32_t slots[kRowSlots][kMaxRowWaves];
   const int64_t b = blockIdx.x / p.L, l = blockIdx.x - b * p.L;
   const int first = threadIdx.x * 8, step = blockDim.x * 8;
   RowValues<XD, YM, NV> r;
@@ -434,7 +465,7 @@ __global__ __launch_bounds__(kMaxRowWaves * 64) void row_norm_kernel(BlockNormPa
 template <int XD, int YM, int NV>
 __global__ __launch_bounds__(512) void staged_row_kernel(BlockNormParams p, int waves, int turns) {
   extern __shared__ __attribute__((aligned(16))) float staged[];
-  __shared__ uint32_t slots[8][2][5][kMaxRowWaves];
+  __shared__ uint32_t slots[8][2][kRowSlots][kMaxRowWaves];
   const int64_t b = blockIdx.y;
   const DirectParams from{p, b, 0};
   for (int c = threadIdx.x * 8; c < p.stage_half * 2; c += 512 * 8) {
@@ -476,26 +507,31 @@ __global__ __launch_bounds__(256) void wide_row_kernel(BlockNormParams p) {
   const float inv_c = 1.0f / (float)p.C;
   const int64_t xo = b * p.xb + l * p.xl, yo = b * p.yb + l * p.yl;
 
-  float y_mean = 0.0f, y_rstd = 1.0f;
-  if (p.y && p.post_norm) {
+  // mean, what is left of it in the centred values, and 1 / sqrt(var + eps), of get(c); as in norm_row
+  auto statistics = [&](int kind, float eps, auto get, float& mean, float& rest, float& rstd) {
     float s = 0.0f;
-    if (p.post_norm == QATTN_NORM_LAYER) {
-      for (int c = lane; c < p.C; c += 64) s += load_elem(p.y, p.y_dtype, yo + c);
-      y_mean = wave_sum(s) * inv_c;
+    if (kind == QATTN_NORM_LAYER) {
+      for (int c = lane; c < p.C; c += 64) s += get(c);
+      mean = wave_sum(s) / (float)p.C;
+      s = 0.0f;
     }
-    s = 0.0f;
+    float var = 0.0f;
     for (int c = lane; c < p.C; c += 64) {
-      const float d = load_elem(p.y, p.y_dtype, yo + c) - y_mean;
-      s = fmaf(d, d, s);
+      const float d = get(c) - mean;
+      s += d, var = fmaf(d, d, var);
     }
-    y_rstd = 1.0f / sqrtf(wave_sum(s) * inv_c + p.post_eps);
-  }
+    if (kind == QATTN_NORM_LAYER) rest = wave_sum(s) / (float)p.C;
+    rstd = inv_deviation(wave_sum(var) * inv_c, rest, eps);
+  };
+  float y_mean = 0.0f, y_rest = 0.0f, y_rstd = 1.0f;
+  if (p.y && p.post_norm)
+    statistics(p.post_norm, p.post_eps, [&](int c) { return load_elem(p.y, p.y_dtype, yo + c); }, y_mean, y_rest, y_rstd);
   auto value = [&](int c) {
     float v = load_elem(p.x, p.x_dtype, xo + c);
     if (p.y) {
       float t = load_elem(p.y, p.y_dtype, yo + c);
       if (p.post_norm) {
-        t = (t - y_mean) * y_rstd;
+        t = (t - y_mean - y_rest) * y_rstd;
         if (p.post_weight.p) t *= load_param(p.post_weight, b, l, c);
         if (p.post_bias.p) t += load_param(p.post_bias, b, l, c);
       }
@@ -508,22 +544,10 @@ __global__ __launch_bounds__(256) void wide_row_kernel(BlockNormParams p) {
     for (int c = lane; c < p.C; c += 64) store_elem(p.h, p.x_dtype, row * p.C + c, value(c));
   if (!p.z) return;
 
-  float mean = 0.0f, rstd = 1.0f;
-  if (p.norm) {
-    float s = 0.0f;
-    if (p.norm == QATTN_NORM_LAYER) {
-      for (int c = lane; c < p.C; c += 64) s += value(c);
-      mean = wave_sum(s) * inv_c;
-    }
-    s = 0.0f;
-    for (int c = lane; c < p.C; c += 64) {
-      const float d = value(c) - mean;
-      s = fmaf(d, d, s);
-    }
-    rstd = 1.0f / sqrtf(wave_sum(s) * inv_c + p.eps);
-  }
+  float mean = 0.0f, rest = 0.0f, rstd = 1.0f;
+  if (p.norm) statistics(p.norm, p.eps, value, mean, rest, rstd);
   auto out = [&](int c) {
-    float z = (value(c) - mean) * rstd;
+    float z = (value(c) - mean - rest) * rstd;
     if (p.weight.p) z *= load_param(p.weight, b, l, c);
     if (p.bias.p) z += load_param(p.bias, b, l, c);
     if (p.scale.p) z = fmaf(z, load_param(p.scale, b, l, c), z);
@@ -582,7 +606,7 @@ static bool row_shape(int C, bool plain, int& waves, int& groups) {
 // 685 / 516).
 constexpr int64_t kStagedRows = 16384;
 constexpr int kStagedWidest = 8192;
-constexpr size_t kLds = 163840, kSlotBytes = 8 * 2 * 5 * kMaxRowWaves * 4;
+constexpr size_t kLds = 163840, kSlotBytes = 8 * 2 * kRowSlots * kMaxRowWaves * 4;
 // Groups a thread holds in the staged kernel, before a row takes two or four waves.
 constexpr int staged_groups(int dtype, int ymode) { return dtype == QATTN_F32 || ymode == Y_F32 ? 3 : 5; }
 constexpr int64_t kCus = 256;
