@@ -68,6 +68,13 @@ __device__ __forceinline__ float activate(float y) {
   }
 }
 
+// A sum with its scales and bias.  The weight's scale comes first: the sum is a whole number below 2^31, so that the product
+// neither overflows nor loses bits below the smallest normal value with any normal scale up to 2^96, and a row's scale, which
+// large or tiny activations bring near either end, meets it where the result itself leaves the range.
+__device__ __forceinline__ float scaled(int sum, float w_scale, float x_scale, float bias) {
+  return fmaf((float)sum * w_scale, x_scale, bias);
+}
+
 // Waits until at most N of the wave's vector memory operations are under way, then for the other waves; the LDS reads
 // too: a fragment read still in flight must not meet the next DMA into its stage.
 template <int N>
@@ -280,7 +287,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         float y[8];
 #pragma unroll
         for (int e = 0; e < 8; e++)
-          y[e] = activate<ACT>(fmaf((float)acc[i + e / 4][j][e % 4] * sx, sw[e / 4][e % 4], bi[e / 4][e % 4]));
+          y[e] = activate<ACT>(scaled(acc[i + e / 4][j][e % 4], sw[e / 4][e % 4], sx, bi[e / 4][e % 4]));
         store_out8(out + 16 * i * es, p.out_dtype, p.N - n0 - cl - 16 * i, y);
       }
     }
@@ -317,8 +324,7 @@ __global__ __launch_bounds__(256) void linear_join_kernel(LinearParams p, int sp
   float y[8];
 #pragma unroll
   for (int e = 0; e < 8; e++)
-    y[e] = e < left ? activate<ACT>(fmaf((float)sum[e / 4][e % 4] * sx, p.w_scale[n0 + e], p.bias ? p.bias[n0 + e] : 0.0f))
-                    : 0.0f;
+    y[e] = e < left ? activate<ACT>(scaled(sum[e / 4][e % 4], p.w_scale[n0 + e], sx, p.bias ? p.bias[n0 + e] : 0.0f)) : 0.0f;
   store_out8(static_cast<char*>(p.out) + (m * p.out_stride + n0) * es, p.out_dtype, left, y);
 }
 
@@ -479,7 +485,7 @@ __global__ __launch_bounds__(512) void linear_few_kernel(FewParams f) {
 #pragma unroll
   for (int e = 0; e < 4; e++)
     if (c + e < p.N) {
-      const float y = activate<ACT>(fmaf((float)sum[e] * sx, sw[e], bias[e]));
+      const float y = activate<ACT>(scaled(sum[e], sw[e], sx, bias[e]));
       const int64_t at = m * p.out_stride + c + e;
       if (p.out_dtype == QATTN_F32) static_cast<float*>(p.out)[at] = y;
       else static_cast<uint16_t*>(p.out)[at] = p.out_dtype == QATTN_FP16 ? f32_to_f16(y) : f32_to_bf16(y);
