@@ -51,7 +51,8 @@ class Int8Weight:
 
     @classmethod
     def quantize(cls, weight: torch.Tensor, bias: Optional[torch.Tensor] = None) -> "Int8Weight":
-        """From a floating weight [N, K] on the GPU: per row, scale = max|w| / 127 and codes = round(127 w / max|w|)."""
+        """From a floating weight [N, K] on the GPU: per row, scale = max|w| / 127 and codes = round(127 w / max|w|).  The
+        weight and the bias are detached: a module's parameters go in as they are."""
         if weight.dim() != 2:
             raise ValueError(f"weight must be [N, K], got {tuple(weight.shape)}")
         rows = per_token_int8(weight.detach())

@@ -9,7 +9,7 @@ reads and writes the whole residual stream.  Here they are one pass over the row
 ``gated_residual_norm``  both: (h, z), z from the float32 h before it is rounded
 ``per_token_int8``       INT8 rows of an activation (or of a weight), one scale per row
 
-Forward only, like the attention they surround: inputs that need a gradient are refused.
+Forward only, like the attention they surround: inputs that need a gradient, or carry a tangent, are refused.
 """
 
 from __future__ import annotations
@@ -17,6 +17,7 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -45,6 +46,10 @@ def _no_grad(*tensors) -> None:
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise ValueError("no backward: call under torch.no_grad() or detach the inputs")
+    if forward_ad._current_level >= 0:  # (a tangent has neither requires_grad nor a part in no_grad)
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError("no forward-mode derivative: detach the inputs")
 
 
 def _check_input(x: torch.Tensor, name: str) -> int:
