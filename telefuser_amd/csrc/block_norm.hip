@@ -630,7 +630,8 @@ static size_t stage(BlockNormParams& p, const Param* const* params) {
 template <int XD, int YM>
 static void launch_rows(const BlockNormParams& p, int waves, int groups, size_t lds, hipStream_t stream) {
   if (lds) {
-    const int vecs = (p.C + 511) / 512, nvmax = staged_groups(XD, YM);
+    constexpr int nvmax = staged_groups(XD, YM);
+    const int vecs = (p.C + 511) / 512;  // at most 16 (kStagedWidest), so four waves hold up to four groups
     const int w = vecs <= nvmax ? 1 : vecs <= 2 * nvmax ? 2 : 4, nv = (vecs + w - 1) / w;
     // rows of a batch entry in turns, as many workgroups as the CUs hold at once: two to a CU by their registers
     const int64_t batches = p.rows / p.L, per = 8 / w;
@@ -641,7 +642,7 @@ static void launch_rows(const BlockNormParams& p, int waves, int groups, size_t 
     else if (nv == 2) staged_row_kernel<XD, YM, 2><<<grid, block, lds, stream>>>(p, w, (int)turns);
     else if (nv == 3) staged_row_kernel<XD, YM, 3><<<grid, block, lds, stream>>>(p, w, (int)turns);
     else if (nv == 4) staged_row_kernel<XD, YM, 4><<<grid, block, lds, stream>>>(p, w, (int)turns);
-    else staged_row_kernel<XD, YM, 5><<<grid, block, lds, stream>>>(p, w, (int)turns);
+    else if constexpr (nvmax > 4) staged_row_kernel<XD, YM, 5><<<grid, block, lds, stream>>>(p, w, (int)turns);
     return;
   }
   if (p.C <= 256) {

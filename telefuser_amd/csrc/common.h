@@ -199,11 +199,6 @@ __device__ __forceinline__ uint32_t wave_reduce(uint32_t v, uint32_t zero, OP op
   v = op(v, dpp<0x143, 0xc>(zero, v));
   return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
-__device__ __forceinline__ float wave_total(float v) {
-  return __uint_as_float(wave_reduce(__float_as_uint(v), 0u, [](uint32_t a, uint32_t b) {
-    return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
-  }));
-}
 __device__ __forceinline__ uint32_t wave_top(uint32_t v) {
   return wave_reduce(v, 0u, [](uint32_t a, uint32_t b) { return max(a, b); });
 }
