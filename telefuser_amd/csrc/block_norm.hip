@@ -7,16 +7,19 @@
 //   n(v) = v | (v - mean) / sqrt(var + eps) | v / sqrt(mean(v^2) + eps)
 //   z is stored in bf16 / fp16 / fp32, or as INT8: code = rint(127 z / max|z|), row scale max|z| / 127
 //
-// Everything between the loads and the stores is fp32; v reaches the norm unrounded.  The variance is that of the
-// centred values.  Parameters are read with the strides of their broadcast shape.
+// Everything between the loads and the stores is fp32; v reaches the norm unrounded.  LayerNorm's mean is removed twice, the
+// second time as what is left of it in the centred values, and the variance is that of the result.  Parameters are read with
+// the strides of their broadcast shape.  A float32 y (a product that is not to be rounded before the sum) takes twice the
+// bytes of a half one: gated residual + norm of 32760 x 1536 74 us, with a float32 y 95 (5.3 TB/s).
 //
 // Bound by memory: x (and y) read once, h and z written once.  At the rate of a copy (5.1 TB/s for 1 GiB) or above where
-// the caches help: gated residual + norm of 75600 x 5120 bf16 0.58 ms (5.3 TB/s), norm of it 306 us (5.1), norm of
-// 32760 x 1536 34 us, row quantizer of 75600 x 5120 206 us (5.6).  What it took: every value loaded once and held in
-// registers (8.4 ms with the row read again for each reduction); reductions over DPP instead of LDS; 16-byte accesses at any
-// alignment (20000 x 5119, one element a load: 405 us, now 130); several narrow rows a wave (75600 x 64: 25 us, now 7);
-// parameters in LDS for many rows; and few VALU instructions a value, which INT8 output has most of: masks only in groups
-// that the row's end cuts, one fused multiply-add for a code of a normalized value (20000 x 5120 to INT8: 110 us, now 88).
+// the caches help (medians, inputs in turn): gated residual + norm of 75600 x 5120 bf16 0.58 ms (5.3 TB/s), modulated norm of
+// it 304 us (5.1), of 32760 x 1536 36 us (from memory 42), row quantizer of 75600 x 5120 210 us (5.5).  What it took: every
+// value loaded once and held in registers (8.4 ms with the row read again for each reduction); reductions over DPP instead of
+// LDS; 16-byte accesses at any alignment (20000 x 5119, one element a load: 405 us, now 131); several narrow rows a wave
+// (75600 x 64: 25 us, now 7.6); parameters in LDS for many rows; and few VALU instructions a value, which INT8 output has
+// most of: masks only in groups that the row's end cuts, one fused multiply-add for a code of a normalized value (20000 x
+// 5120 to INT8: 110 us, then 85, and 92 with the second part of the mean).
 #include "attn_device.h"
 
 namespace qattn {
@@ -497,7 +500,9 @@ __global__ __launch_bounds__(512) void staged_row_kernel(BlockNormParams p, int 
 }
 
 // ------------------------------------------------------------------------------------------------
-// rows too wide for that: one wave per row, one element per lane and step, the row read again for each reduction
+// rows too wide for that: one wave per row, one element per lane and step, the row read again for each reduction, and codes
+// from the corrected quotient for normalized values too.  The simple kernel that the others replaced, kept for widths that
+// the framework's models do not have: latency of a row's steps bounds it (quantizer of 1 x 28672 228 us, of 500 x 28672 399).
 // ------------------------------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void wide_row_kernel(BlockNormParams p) {
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -588,7 +593,7 @@ static int check_param(const qattn_param& q, const char* name, int64_t B, int64_
 // waves.  A thread that has only x to read takes up to 5 groups, and a wave more costs as much as 12 lanes' worth of groups:
 // reductions between waves take barriers (row quantizer of 39606 x 3328 with 7 / 4 / 3 / 2 waves: 134 / 99 / 96 / 79 us).
 // One that reads y or parameters beside it takes 2 where 8 waves suffice: its registers then leave room for more waves
-// (2 x 4680 x 5120, 5 / 2 groups at most: norm with per-token scale and shift 113 / 108 us).
+// (2 x 4680 x 5120, 5 / 2 groups at most: norm with per-token scale and shift 113 / 106 us).
 static bool row_shape(int C, bool plain, int& waves, int& groups) {
   const int vecs = (C + 7) / 8;
   int64_t best = -1;
@@ -601,9 +606,12 @@ static bool row_shape(int C, bool plain, int& waves, int& groups) {
   return best >= 0;
 }
 
-// Staging pays from about this many rows of a batch entry (microseconds, read per row / staged: norm of 9000 x 5120 38.7 /
-// 43.7, of 20000 x 5120 96 / 85, of 75600 x 5120 365 / 306; gated residual + norm of 75600 x 640 111 / 85, of 48306 x 7040
-// 685 / 516).
+// Staging pays for many rows of a batch entry (microseconds, read per row / staged: norm of 4680 x 5120 26 / 30, of 9000 x
+// 5120 45.5 / 45 from one input that the caches hold and 53 / 47 from several in turn, of 16384 x 5120 95 / 75, of 75600 x
+// 5120 429 / 304, of 16384 x 1536 26 / 19; gated residual + norm of 75600 x 640 109 / 83, of 48306 x 7040 600 / 514).  The
+// two are equal at about 9000 rows already: between that and this number some calls take up to a fifth longer than they
+// could.  A batch entry counts by itself: 21 frames of 1560 x 1536 with parameters of their own read them for every row (62
+// us, as one entry of 32760 rows 36).
 constexpr int64_t kStagedRows = 16384;
 constexpr int kStagedWidest = 8192;
 constexpr size_t kLds = 163840, kSlotBytes = 8 * 2 * kRowSlots * kMaxRowWaves * 4;
@@ -633,7 +641,9 @@ static void launch_rows(const BlockNormParams& p, int waves, int groups, size_t 
     constexpr int nvmax = staged_groups(XD, YM);
     const int vecs = (p.C + 511) / 512;  // at most 16 (kStagedWidest), so four waves hold up to four groups
     const int w = vecs <= nvmax ? 1 : vecs <= 2 * nvmax ? 2 : 4, nv = (vecs + w - 1) / w;
-    // rows of a batch entry in turns, as many workgroups as the CUs hold at once: two to a CU by their registers
+    // rows of a batch entry in turns, by two workgroups for each CU where LDS holds them.  Kernels of more than 128 registers
+    // (four groups a thread or more, three with y) have room for one at a time: the second half of their grid then follows
+    // the first and stages the parameters once more.
     const int64_t batches = p.rows / p.L, per = 8 / w;
     const int64_t hold = std::max((int64_t)1, kCus * std::min((int64_t)2, (int64_t)(kLds / (lds + kSlotBytes))) / batches);
     const int64_t turns = (p.L + per * hold - 1) / (per * hold);

@@ -23,9 +23,14 @@
 // 64, four (39606 x 64 x 3328 26.5 us, with three 28.1), where larger ones leave CUs without work.  A stage of the 128 x 128
 // tile takes about 950 cycles for 512 of MFMA; reads, DMA and MFMAs overlap in part (without the MFMAs 32.4 of 34.5 us at
 // 1560 x 1536 x 8960, without the LDS reads 29.4, without the DMA 25.8).  96 x 128 tiles, on 204 CUs there instead of 156,
-// fetch a seventh more in all and take the same time.  The tiny tile fetches twice as much for its products.  Rows past M or
-// N lie behind the end of the buffer resource and read as zeros; so does every stage past the last.
-// 75600 x 13824 x 5120 4.10 ms (2.61 PFLOP/s), 32760 x 1536 x 8960 377 us (2.40), 32760 x 4608 x 1536 208 us (2.23).
+// fetch a seventh more in all and take the same time.  The tiny tile fetches twice as much for its products, and runs one
+// workgroup a CU as all of them do: two waves a SIMD is what the large tile's registers allow, and the attribute that says so
+// holds for every instantiation, though this one's 54 registers and 67 KiB of LDS have room for two.  Rows past M or N lie
+// behind the end of the buffer resource and read as zeros, and so does every stage past the last (the range check counts the
+// scalar offset, and does not wrap where that is past the end).
+// 75600 x 13824 x 5120 4.16 ms (2.57 PFLOP/s, the least of 30 launches 4.10 and 2.61), with GELU 4.23; one call after the
+// other, 32760 x 1536 x 8960 365 us (2.47), 32760 x 4608 x 1536 212 us (2.19).  The power that a product takes depends on its
+// values: launches apart from each other on codes spread evenly over the whole range take up to a third longer.
 #include "attn_device.h"
 
 namespace qattn {
@@ -551,7 +556,8 @@ static int linear_params(LinearParams& p, const int8_t* w, int64_t w_pitch, cons
 // Which kernel, by estimated microseconds: of a stage and of a tile's beginning and end, times the rounds of the chip; a
 // split along K writes its int32 sums and the join reads them (5 TB/s, and 3 us for its launch).  Measured, large / small /
 // tiny tile: 3000 x 3000 x 3000 38 / 42 / -, 32760 x 4608 x 1536 208 / 338 / -, 1560 x 1536 x 8960 85 / 30 / 46, 512 x 5120 x
-// 4096 43 / 17 / 26, 600 x 1536 x 1536 19 / 8.3 / 6.1, 777 x 999 x 1027 - / 9.7 / 5.7, 1000 x 640 x 4096 - / 15.6 / 9.6.
+// 4096 43 / 17 / 26, 600 x 1536 x 1536 19 / 8.3 / 6.1, 777 x 999 x 1027 - / 9.7 / 5.7, 1000 x 640 x 4096 - / 15.6 / 9.6; all
+// with one workgroup a CU, which the rounds count too.
 enum LinearKernel { LINEAR_FEW, LINEAR_LARGE, LINEAR_SMALL, LINEAR_TINY };
 struct LinearPlan {
   LinearKernel kernel;
